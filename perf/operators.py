@@ -80,7 +80,7 @@ def _logint(rng, lo, hi):
 def draw(rng):
     op = rng.choice(["attention", "attention", "norm", "dropout"])
     if op == "attention":
-        d = rng.choice([32, 32, 64, 64, 128])
+        d = rng.choice([16, 32, 32, 64, 64])
         hk = rng.choice([1, 2])
         h = hk * rng.choice([1, 1, 2, 4])
         b = rng.choice([1, 2, 3])
