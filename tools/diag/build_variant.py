@@ -18,7 +18,7 @@ def main():
         if f.endswith(".hip"):
             o = os.path.join(objdir, f[:-4] + ".o")
             objs.append(o)
-            procs.append(subprocess.Popen(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + flags
+            procs.append(subprocess.Popen(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + flags
                                           + ["-c", os.path.join(csrc, f), "-o", o]))
     assert all(p.wait() == 0 for p in procs)
     out = os.path.join(PKG, "lib", "libvspw_hip_%s.so" % name)
