@@ -83,6 +83,60 @@ class SynchronizedBatchNorm3d(_SynchronizedBatchNorm):
 BatchNorm2d = SynchronizedBatchNorm2d
 
 
+class _CounterRng:
+    """(seed, offset) state of a dropout layer: a non-persistent int64 buffer, the seed drawn from torch's CPU generator at
+    construction.  draw() hands out the state of this step and advances the offset on the stream (graph-safe)."""
+
+    def _init_rng(self):
+        self.register_buffer("rng_state", torch.stack((torch.randint(0, 2 ** 62, ()), torch.zeros((), dtype=torch.int64))),
+                             persistent=False)
+
+    def manual_seed(self, seed, offset=0):
+        self.rng_state.copy_(torch.tensor([int(seed), int(offset)], dtype=torch.int64))
+        return self
+
+    def draw(self):
+        return ops.rng_next(self.rng_state)
+
+
+class Dropout(nn.Dropout, _CounterRng):
+    """nn.Dropout whose mask is recomputed from a counter-based generator in forward and backward (ops.dropout)."""
+
+    channelwise = False
+
+    def __init__(self, p=0.5):
+        super().__init__(p)
+        self._init_rng()
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        return ops.dropout(x, self.p, self.draw(), self.channelwise)
+
+
+class Dropout2d(nn.Dropout2d, _CounterRng):
+    """nn.Dropout2d from the same generator: whole channels of [N,C,...] are dropped."""
+
+    channelwise = True
+
+    def __init__(self, p=0.5):
+        super().__init__(p)
+        self._init_rng()
+
+    forward = Dropout.forward
+
+
+class GroupNorm(nn.GroupNorm):
+    """nn.GroupNorm on channels-last activations, with the activation and dropout that follow it in the same kernels."""
+
+    def forward(self, x, act="none", dropout=None):
+        if dropout is not None and not isinstance(dropout, _CounterRng):
+            raise NotImplementedError("GroupNorm fuses the counter-based Dropout / Dropout2d of this module only")
+        live = dropout is not None and dropout.training and dropout.p > 0.0
+        return ops.group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, act, dropout.p if live else 0.0,
+                                  dropout.draw() if live else None, live and dropout.channelwise)
+
+
 def dropout2d_mask(module, x_shape, device):
     """Per-(image, channel) keep mask scaled by 1/(1-p) for nn.Dropout2d in training mode, else None.
     `module._forced_mask` (tests) overrides the RNG draw."""
@@ -92,6 +146,8 @@ def dropout2d_mask(module, x_shape, device):
     if forced is not None:
         return forced.to(device=device, dtype=torch.float32).contiguous()
     n, c = x_shape[0], x_shape[1]
+    if isinstance(module, Dropout2d):
+        return ops.dropout(torch.ones((n, c), device=device), module.p, module.draw(), True)
     keep = 1.0 - module.p
     return (torch.rand((n, c), device=device) < keep).float().div_(keep)
 
@@ -117,9 +173,17 @@ class AdaptiveAvgPool2d(nn.AdaptiveAvgPool2d):
         return ops.pyramid_pool(x, (int(s),), 1, None)[0]
 
 
+def _act_name(m):
+    """"relu" / "silu" / "gelu" for the activations group_norm_act evaluates, else None."""
+    if isinstance(m, nn.GELU):
+        return "gelu" if m.approximate == "none" else None
+    return "relu" if isinstance(m, nn.ReLU) else "silu" if isinstance(m, nn.SiLU) else None
+
+
 class FusedSequential(nn.Sequential):
     """nn.Sequential (same child indices, hence same state_dict keys) whose forward fuses
-    Conv2d -> BatchNorm -> ReLU -> Dropout2d runs into single kernels chains."""
+    Conv2d -> BatchNorm -> ReLU -> Dropout2d and GroupNorm -> ReLU / SiLU / GELU -> Dropout / Dropout2d runs into single
+    kernels chains."""
 
     def forward(self, x):
         mods = list(self)
@@ -148,8 +212,18 @@ class FusedSequential(nn.Sequential):
                 mask = dropout2d_mask(drop, x.shape, x.device)
                 x = m(x, relu=relu, mask=mask)
                 i = j
-            elif isinstance(m, (nn.ReLU, nn.Dropout2d)):
-                raise NotImplementedError("bare %s outside a BatchNorm chain is not on the VSPW hot path"
+            elif isinstance(m, GroupNorm):
+                j = i + 1
+                act = _act_name(mods[j]) if j < len(mods) else None
+                if act is not None:
+                    j += 1
+                drop = mods[j] if j < len(mods) and isinstance(mods[j], _CounterRng) else None
+                if drop is not None:
+                    j += 1
+                x = m(x, act or "none", drop)
+                i = j
+            elif isinstance(m, (nn.ReLU, nn.Dropout2d)) and not isinstance(m, _CounterRng):
+                raise NotImplementedError("bare %s outside a normalisation chain is not on the VSPW hot path"
                                           % type(m).__name__)
             else:
                 x = m(x)

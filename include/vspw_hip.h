@@ -29,6 +29,12 @@ extern "C" {
 #define VSPW_EINVAL (-1)  /* bad argument / geometry / workspace too small */
 #define VSPW_ELAUNCH (-2) /* hipLaunchKernel reported an error */
 
+/* Element types of the operators that take 16-bit activations (group norm, dropout, differential attention); the others
+ * take fp32 only. */
+#define VSPW_F32 0
+#define VSPW_BF16 1
+#define VSPW_F16 2
+
 #define VSPW_ABI_VERSION 7
 int vspw_abi_version(void);
 /* The hipError_t behind the most recent VSPW_ELAUNCH (0 if none) - for error messages. */
@@ -612,6 +618,32 @@ int vspw_xchg_bn_finalize(double* sums, int c, void* const* arenas, int world, i
                           int slot_doubles, double timeout_s, int* status, double count, const float* gamma,
                           const float* beta, float* running_mean, float* running_var, float momentum, float eps,
                           float* mean, float* invstd, float* scale, float* shift, int clamp_var, void* stream);
+
+/* ---------------------------------------------------------------- dropout (dropout.hip) ------------ */
+/* y = x * keep / (1 - p) without a stored mask: keep = [u >= floor(p 2^32)], u = word e % 4 of Philox4x32-10 counter
+ * (e / 4, offset) under key `seed`; rng = (seed, offset), two int64 in DEVICE memory (a captured graph reads them at replay).
+ * x, y: n*hw*c elements of type dtype in [n][hw][c] order; e = the element's index in that order, or image * c + channel
+ * when channelwise != 0 (whole channels: nn.Dropout2d of models/clip_psp.py:33,56).  The same call on the gradient is the
+ * backward pass.  A dropped inf or NaN gives 0; p = 1 drops everything.  x == y is allowed. */
+int vspw_dropout(const void* x, void* y, long long n, long long hw, int c, int dtype, double p, const long long* rng,
+                 int channelwise, void* stream);
+/* used = state; state.offset += 1, in stream order: the (seed, offset) of one training step of a dropout layer. */
+int vspw_rng_next(long long* state, long long* used, void* stream);
+
+/* ---------------------------------------------------------------- group norm (group_norm.hip) ------ */
+/* y = drop(act(w (x - mean) / sqrt(var + eps) + b)) on [n][hw][c] activations of type dtype, mean / var over the hw pixels and
+ * the c / groups channels of a group; w, b (fp32 [c]) may be NULL; act 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf); p, rng,
+ * channelwise as vspw_dropout (p = 0: none, rng may be NULL).  stats [n][groups][2] (fp64 mean and 1/sqrt(var + eps)) is
+ * what the backward pass reads; NULL at inference.  16-byte aligned pointers where c is a multiple of 16 bytes. */
+size_t vspw_group_norm_fwd_workspace(int n, long long hw, int c, int groups, int dtype);
+int vspw_group_norm_fwd(const void* x, void* y, int n, long long hw, int c, int groups, int dtype, const float* w,
+                        const float* b, float eps, int act, double p, const long long* rng, int channelwise, double* stats,
+                        void* ws, size_t ws_bytes, void* stream);
+/* dx, dw, db (each may be NULL) from dy, the forward input and its stats; the dropout mask is regenerated. */
+size_t vspw_group_norm_bwd_workspace(int n, long long hw, int c, int groups, int dtype);
+int vspw_group_norm_bwd(const void* x, const void* dy, void* dx, int n, long long hw, int c, int groups, int dtype,
+                        const float* w, const float* b, int act, double p, const long long* rng, int channelwise,
+                        const double* stats, float* dw, float* db, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
