@@ -9,7 +9,7 @@ There is no CPU fallback: a CPU tensor raises (SURVEY.md §8b "Errors").
 
 Layout of the module family: _opbase.py (pointer / layout helpers, launch timers), _ops_conv.py (convolutions, Winograd
 dispatch, derived-weight caches), _ops_bn.py (BatchNorm, conv+BN+activation nodes), _ops_norm.py (GroupNorm+activation,
-counter-based dropout: also bfloat16 / float16); this file holds the remaining operators (pooling, interpolation, losses, batched GEMMs, non-local, flow) and re-exports the others, so callers keep
+counter-based dropout: also bfloat16 / float16), _ops_attn.py (differential attention: also bfloat16); this file holds the remaining operators (pooling, interpolation, losses, batched GEMMs, non-local, flow) and re-exports the others, so callers keep
 using `ops.<name>`.
 """
 import ctypes
@@ -34,6 +34,8 @@ from ._ops_bn import (  # noqa: F401 (re-exported: callers use ops.<name>)
     _decisions, _finalize_name, _infer_fold, _sync_finalize, _sync_group, _sync_world, batch_norm_act,
     conv_bn_act, invalidate_inference_cache, materialize, record_decisions, set_bn_backward_fusion,
     set_inference_folding, set_sync_bn, sync_bn_timer)
+from ._ops_attn import (  # noqa: F401 (re-exported)
+    DiffAttentionFn, DiffLambdaFn, diff_attention, diff_attention_supported, diff_lambda)
 from ._ops_norm import DropoutFn, GroupNormActFn, dropout, group_norm_act, rng_next  # noqa: F401 (re-exported)
 
 

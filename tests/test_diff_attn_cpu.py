@@ -1,0 +1,88 @@
+"""Host side of differential attention: refusals, the descriptor and the workspace arithmetic (no GPU)."""
+import ctypes
+import itertools
+
+import pytest
+import torch
+
+
+def desc(**kw):
+    from cvpr2021_vspw_implement_amd._ops_attn import AttnDesc
+
+    a = dict(b=1, nq=10, nk=20, h=4, hk=2, d=32, dtype=0, lam_dtype=0, frame=0, scale=0.2)
+    a.update(kw)
+    s = dict(q_sb=0, q_sn=a["h"] * 64, q_sh=64, q_sm=32, k_sb=0, k_sn=a["hk"] * 64, k_sh=64, k_sm=32, v_sb=0, v_sn=a["hk"] * 64,
+             v_sh=64)
+    return AttnDesc(*[a[n] for n, _ in AttnDesc._fields_[:10]], *s.values())
+
+
+def test_cpu_tensors_are_refused():
+    from cvpr2021_vspw_implement_amd import ops
+
+    with pytest.raises(RuntimeError):
+        ops.diff_attention(torch.ones(1, 2, 1, 2, 16), torch.ones(1, 2, 1, 2, 16), torch.ones(1, 2, 1, 32), torch.ones(1))
+    with pytest.raises(RuntimeError):
+        ops.diff_lambda(*[torch.ones(1, 4)] * 4, 0.1)
+
+
+def test_the_descriptor_matches_the_header():
+    """Field order and types of the ctypes structure against the struct in the header."""
+    import re
+
+    from cvpr2021_vspw_implement_amd import _C
+    from cvpr2021_vspw_implement_amd._ops_attn import AttnDesc
+
+    body = re.search(r"typedef struct vspw_dattn_desc \{(.*?)\}", open(_C.HEADER).read(), re.S).group(1)
+    fields = []
+    for line in body.split(";"):
+        m = re.match(r"\s*(int|float|long long)\s+(.*)", line, re.S)
+        if m:
+            ty = {"int": ctypes.c_int, "float": ctypes.c_float, "long long": ctypes.c_longlong}[m.group(1)]
+            fields += [(n.strip(), ty) for n in m.group(2).split(",")]
+    assert fields == AttnDesc._fields_
+
+
+def test_c_entry_points_refuse_bad_arguments():
+    """Every refusal comes before a launch; the pointers are never followed."""
+    from cvpr2021_vspw_implement_amd import _C
+
+    lib = _C.load()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4100)
+
+    def fwd(d=None, q=p, k=p, v=p, lam=p, out=p, ws=p, n=1 << 30):
+        return lib.vspw_diff_attn_fwd(ctypes.byref(d or desc()), q, k, v, lam, None, out, None, None, ws, n, None)
+
+    bad = [dict(b=0), dict(nq=0), dict(nk=0), dict(h=3), dict(hk=0), dict(d=48), dict(d=8), dict(dtype=2), dict(lam_dtype=2),
+           dict(frame=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(nq=2 ** 31 - 1),
+           dict(nk=2 ** 31 - 1), dict(b=2 ** 30, nq=2 ** 20)]
+    for kw in bad:
+        assert fwd(desc(**kw)) == -1, kw
+        assert _C.query("vspw_diff_attn_fwd_workspace", ctypes.byref(desc(**kw))) == 0
+        assert _C.query("vspw_diff_attn_bwd_workspace", ctypes.byref(desc(**kw))) == 0
+    for kw in (dict(q=None), dict(k=None), dict(v=None), dict(lam=None), dict(out=None), dict(q=odd), dict(v=odd), dict(out=odd)):
+        assert fwd(**kw) == -1, kw
+    strided = desc()
+    strided.k_sn = 130
+    assert fwd(strided) == -1
+    big = desc(nk=20000, nq=1)
+    assert _C.query("vspw_diff_attn_fwd_workspace", ctypes.byref(big)) > 0
+    assert fwd(big, ws=None) == -1 and fwd(big, n=8) == -1 and fwd(big, ws=odd) == -1
+
+    def bwd(d=None, lse=p, o2=p, dk=p, dv=p, ws=p, n=1 << 30):
+        return lib.vspw_diff_attn_bwd(ctypes.byref(d or desc()), p, p, p, p, None, p, o2, lse, p, p, dk, dv, p, ws, n, None)
+
+    for kw in (dict(lse=None), dict(o2=None), dict(dk=None), dict(dv=None), dict(ws=None), dict(n=8), dict(d=desc(d=20))):
+        assert bwd(**kw) == -1, kw
+    assert lib.vspw_diff_lambda_fwd(p, p, p, p, 0.1, None, 1, 4, None) == -1
+    assert lib.vspw_diff_lambda_fwd(p, p, p, p, 0.1, p, 0, 4, None) == -1
+    assert lib.vspw_diff_lambda_bwd(p, p, p, p, None, p, p, p, p, 1, 4, None) == -1
+
+
+def test_workspaces_hold_whole_parts():
+    """The forward workspace is a whole number of parts of every row's two sums, maxima and sums of weights."""
+    from cvpr2021_vspw_implement_amd import _C
+
+    for b, nq, nk, (h, hk), d in itertools.product((1, 3), (1, 33, 900), (1, 40, 5000, 25200), ((1, 1), (8, 2)), (16, 64)):
+        n = _C.query("vspw_diff_attn_fwd_workspace", ctypes.byref(desc(b=b, nq=nq, nk=nk, h=h, hk=hk, d=d)))
+        row = b * h * nq * (4 * d + 4) * 4
+        assert n % row == 0 and n // row != 1 and n // row <= (nk + 31) // 32
