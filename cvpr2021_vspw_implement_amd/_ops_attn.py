@@ -48,7 +48,7 @@ def _pairs(q, k, frame):
 
 
 class DiffAttentionFn(torch.autograd.Function):
-    """Forward keeps out, the second map's output and the log-sum-exp of both maps; backward recomputes the scores."""
+    """Forward keeps both maps' outputs in float32 and their log-sum-exps; backward recomputes the scores."""
 
     @staticmethod
     def forward(ctx, q, k, v, lam, scale, mask, frame):
@@ -57,27 +57,27 @@ class DiffAttentionFn(torch.autograd.Function):
         nk, hk = k.shape[1], k.shape[2]
         train = any(ctx.needs_input_grad[:4])
         out = torch.empty((b, nq, h, 2 * d), device=q.device, dtype=q.dtype)
-        o2 = lse = None
+        maps = lse = None
         if out.numel() and nk:
             with _on(q):
                 if train:
-                    o2 = torch.empty_like(out)
+                    maps = torch.empty((b, nq, h, 2, 2 * d), device=q.device, dtype=torch.float32)
                     lse = torch.empty((2, b * hk, nq * (h // hk)), device=q.device, dtype=torch.float32)
                 ds = _desc(q, k, v, lam, scale, frame)
                 nbytes = _C.query("vspw_diff_attn_fwd_workspace", ctypes.byref(ds))
                 ws = _ws(nbytes, q.device) if nbytes else None
                 with _Timed("diff_attn_fwd", 12.0 * b * h * d * _pairs(q, k, frame), "diff_attn b%d n%d/%d h%d d%d" % (b, nq, nk, h, d)):
-                    _C.call("vspw_diff_attn_fwd", ctypes.byref(ds), _p(q), _p(k), _p(v), _p(lam), _p(mask), _p(out), _p(o2),
+                    _C.call("vspw_diff_attn_fwd", ctypes.byref(ds), _p(q), _p(k), _p(v), _p(lam), _p(mask), _p(out), _p(maps),
                             _p(lse), _p(ws), nbytes, _stream())
         else:
             out.zero_()
         ctx.meta = (scale, frame)
-        ctx.save_for_backward(q, k, v, lam, mask, out, o2, lse)
+        ctx.save_for_backward(q, k, v, lam, mask, maps, lse)
         return out
 
     @staticmethod
     def backward(ctx, go):
-        q, k, v, lam, mask, out, o2, lse = ctx.saved_tensors
+        q, k, v, lam, mask, maps, lse = ctx.saved_tensors
         scale, frame = ctx.meta
         need = ctx.needs_input_grad
         b, nq, h, _, d = q.shape
@@ -87,7 +87,7 @@ class DiffAttentionFn(torch.autograd.Function):
             dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if need[1] or need[2] else None
             dv = torch.empty(v.shape, device=q.device, dtype=q.dtype) if need[1] or need[2] else None
             dlam = torch.empty_like(lam) if need[3] else None
-            if o2 is None:  # no rows or no keys
+            if maps is None:  # no rows or no keys
                 for t in (dq, dk, dv, dlam):
                     if t is not None:
                         t.zero_()
@@ -97,7 +97,7 @@ class DiffAttentionFn(torch.autograd.Function):
                 nbytes = _C.query("vspw_diff_attn_bwd_workspace", ctypes.byref(ds))
                 ws = _ws(nbytes, q.device)
                 with _Timed("diff_attn_bwd", 28.0 * b * h * d * _pairs(q, k, frame), "diff_attn b%d n%d/%d h%d d%d" % (b, nq, nk, h, d)):
-                    _C.call("vspw_diff_attn_bwd", ctypes.byref(ds), _p(q), _p(k), _p(v), _p(lam), _p(mask), _p(out), _p(o2),
+                    _C.call("vspw_diff_attn_bwd", ctypes.byref(ds), _p(q), _p(k), _p(v), _p(lam), _p(mask), _p(maps),
                             _p(lse), _p(go), _p(dq), _p(dk), _p(dv), _p(dlam), _p(ws), nbytes, _stream())
         return dq, dk if need[1] else None, dv if need[2] else None, dlam, None, None, None
 

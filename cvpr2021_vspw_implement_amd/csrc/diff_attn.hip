@@ -17,11 +17,13 @@
 // from the saved log-sum-exp.  Long axes are split over workgroups when there are few rows (or keys); the partial results are
 // joined in a fixed order, so every result is bit-reproducible.
 //
-// All softmax statistics and sums are fp32.  bf16 inputs: P and dS are rounded to bf16 (half a step, 2^-9 relative, of
-// positive weights or of differences whose errors average over the keys) because the matrix unit takes both operands in the
-// same type; everything else stays fp32 until the one rounding of each result.
+// All softmax statistics and sums are fp32.  bf16 inputs: P and dS enter the matrix unit, which takes both operands in the same
+// type, as two bf16 terms (16 bits: rounded to one term alone they cost as much as the rounding of the result does, measured
+// 2.4e-3 against 1.7e-3 relative); everything else stays fp32 until the one rounding of each result.
 #include <limits.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "elem.h"
 
@@ -67,7 +69,12 @@ struct Mx<float> {
         }
         return f;
     }
-    static __device__ __forceinline__ Frag reg(const f32x16& s, int t) {
+    typedef Frag RegFrag;
+    static constexpr int STEPS = 8, RSTEPS = 8;  // matrix instructions per product of two fragments
+    // The frame rule in every tile and the scores of one tile too many are hidden behind the matrix instructions here, and a
+    // second or third copy of the loop costs registers that spill.
+    static constexpr bool ONE_LOOP = true;
+    static __device__ __forceinline__ RegFrag reg(const f32x16& s, int t) {
         Frag f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -76,12 +83,10 @@ struct Mx<float> {
         }
         return f;
     }
-    static __device__ __forceinline__ void mma(f32x16& acc, const Frag& x, const Frag& y) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.a[e], y.a[e], acc, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.b[e], y.b[e], acc, 0, 0, 0);
+    static __device__ __forceinline__ void step(f32x16& acc, const Frag& x, const Frag& y, int e) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(e < 4 ? x.a[e & 3] : x.b[e & 3], e < 4 ? y.a[e & 3] : y.b[e & 3], acc, 0, 0, 0);
     }
+    static __device__ __forceinline__ void rstep(f32x16& acc, const Frag& x, const RegFrag& y, int e) { step(acc, x, y, e); }
     static __device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
 };
 
@@ -107,14 +112,34 @@ struct Mx<bf16_t> {
         const s16x8 ab = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(bf16x8, ab);
     }
-    static __device__ __forceinline__ Frag reg(const f32x16& s, int t) {
-        Frag f;
+    struct RegFrag {
+        Frag hi, lo;
+    };
+    static __device__ __forceinline__ unsigned pack(float x, float y) {  // two at a time: one instruction
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x, y}, bf16x2));
+    }
+    static constexpr int STEPS = 1, RSTEPS = 2;
+    static constexpr bool ONE_LOOP = false;
+    static __device__ __forceinline__ RegFrag reg(const f32x16& s, int t) {
+        u32x4 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (bf16_t)s[8 * t + e];
+        for (int i = 0; i < 4; ++i) {
+            const float x = s[8 * t + 2 * i], y = s[8 * t + 2 * i + 1];
+            hi[i] = pack(x, y);
+            lo[i] = pack(x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u));
+        }
+        RegFrag f;
+        f.hi = __builtin_bit_cast(Frag, hi);
+        f.lo = __builtin_bit_cast(Frag, lo);
         return f;
     }
-    static __device__ __forceinline__ void mma(f32x16& acc, const Frag& x, const Frag& y) {
+    static __device__ __forceinline__ void step(f32x16& acc, const Frag& x, const Frag& y, int) {
         acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void rstep(f32x16& acc, const Frag& x, const RegFrag& y, int e) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, e ? y.lo : y.hi, acc, 0, 0, 0);
     }
     static __device__ __forceinline__ void store4(bf16_t* p, f32x4 v) {
         bf16x4 o;
@@ -124,12 +149,18 @@ struct Mx<bf16_t> {
     }
 };
 
+// Holds the order of the instruction stream: the vector work of a tile is dealt out between matrix instructions (64 cycles each
+// in fp32) and operand fragments are read one step ahead; left to itself the compiler moves all reads up and runs out of
+// registers, or gathers the vector work in one place, where the matrix unit waits for it.
+__device__ __forceinline__ void da_pin() { __builtin_amdgcn_sched_barrier(0); }
+
 struct DaArgs {
     const void *q, *k, *v, *lam, *go;
     const unsigned char* mask;
-    void *out, *o2;             // [B,Nq,H,2D]
+    void* out;                  // [B,Nq,H,2D]
+    float* maps;                // [B,Nq,H,2,2D]: P_1 v and P_2 v in fp32, for D_m
     float* lse;                 // [2][B*Hk][rows]: log2-sum-exp2 of s log2(e) S (+inf: no visible key)
-    float* delta;               // [2][B*Hk][rows]: D_m
+    float* stat;                // [6][B*Hk][rows]: both log-sum-exps, D_1, D_2, lambda, key limit (int): a row's constants
     void *dq, *dk, *dv, *dlam;
     float* part;                // partial results of a split axis
     float* ml;                  // forward: [chunks][B*Hk][rows][2] running maximum and sum per map: [..][2 m], [..][2 m + 1]
@@ -138,11 +169,13 @@ struct DaArgs {
     int b, nq, nk, h, hk, g, rows, frame, lam_bf16, lchunks;
     int tiles, parts, span;     // workgroups along the owned axis; split of the streamed axis: parts of `span` entries
     float c, scale;             // scale * log2(e), scale
+    unsigned gm, gs;            // x / g = x * gm >> gs for 0 <= x < 2^31
 };
 
 __device__ __forceinline__ float da_lambda(const DaArgs& a, int head) {
     return a.lam_bf16 ? (float)reinterpret_cast<const bf16_t*>(a.lam)[head] : reinterpret_cast<const float*>(a.lam)[head];
 }
+__device__ __forceinline__ int da_div(const DaArgs& a, int x) { return (int)(((unsigned long long)(unsigned)x * a.gm) >> a.gs); }
 // keys [0, lim) are within the frames that the row's query sees
 __device__ __forceinline__ int da_limit(const DaArgs& a, int row) {
     if (!a.frame) return a.nk;
@@ -157,52 +190,141 @@ __device__ __forceinline__ f32x16 zero16() {
     for (int r = 0; r < 16; ++r) z[r] = 0.f;
     return z;
 }
+// maximum over the two lane halves
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ int acc_index(int r, int lh) { return (r & 3) + 8 * (r >> 2) + 4 * lh; }
+__device__ __forceinline__ f32x4 quad(const f32x16& s, int g4) { return f32x4{s[4 * g4], s[4 * g4 + 1], s[4 * g4 + 2], s[4 * g4 + 3]}; }
 
-// Streams [32][2D] tiles of two tensors (k and v, or q and dO) through registers into LDS: 16-byte vectors, thread t moves
-// number t + threads * i; entries that take no part arrive as zeros whatever their memory holds.
+// A streamed [32][2D] tile on its way from global memory through registers into LDS: 16-byte vectors, thread t moves the
+// vectors t + THREADS * i (a tile smaller than the workgroup is moved more than once).  Nothing here branches or looks at what
+// a load brought before put(): a branch would part the vector work from the matrix instructions it is dealt out between, a
+// look would wait for memory.
 template <typename T, int D, int THREADS>
 struct Stager {
     static constexpr int VE = 16 / (int)sizeof(T);
-    static constexpr int VROW = 2 * D / VE;             // vectors per row
+    static constexpr int VROW = 2 * D / VE;  // vectors per row
     static constexpr int TOTAL = DA_TILE * VROW;
     static constexpr int F = (TOTAL + THREADS - 1) / THREADS;
+    static constexpr int STEP = THREADS / VROW;  // rows between a thread's vectors
     static constexpr int LD = 2 * D + Mx<T>::PAD;
-    u32x4 x[F], y[F];
+    static_assert((TOTAL % THREADS == 0 || THREADS % TOTAL == 0) && THREADS % VROW == 0, "");
+    u32x4 x[F];
 
-    template <typename PX, typename PY>
-    __device__ __forceinline__ void load(int tid, PX px, PY py) {  // p?(row of the tile, column, ok) -> address
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-            const int idx = tid + THREADS * i;
-            const int row = TOTAL % THREADS == 0 || idx < TOTAL ? idx / VROW : 0;
-            const int col = (idx % VROW) * VE;
-            bool ok;
-            const T* a = px(row, col, ok);
-            const T* b = py(row, col);
-            const u32x4 va = *reinterpret_cast<const u32x4*>(a), vb = *reinterpret_cast<const u32x4*>(b);
-            const u32x4 z = {0, 0, 0, 0};
-            x[i] = ok ? va : z;
-            y[i] = ok ? vb : z;
-        }
-    }
-    __device__ __forceinline__ void store(int tid, T* X, T* Y) const {
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-            const int idx = tid + THREADS * i;
-            if (TOTAL % THREADS == 0 || idx < TOTAL) {
-                const int o = (idx / VROW) * LD + (idx % VROW) * VE;
-                *reinterpret_cast<u32x4*>(X + o) = x[i];
-                *reinterpret_cast<u32x4*>(Y + o) = y[i];
-            }
-        }
+    static __device__ __forceinline__ int row(int tid, int i) { return tid % TOTAL / VROW + STEP * i; }
+    static __device__ __forceinline__ int col(int tid) { return tid % VROW * VE; }
+    __device__ __forceinline__ void get(int i, const char* base, unsigned off) { x[i] = *reinterpret_cast<const u32x4*>(base + off); }
+    __device__ __forceinline__ void put(int tid, int i, T* X, bool ok) const {  // rows that take no part: zeros
+        *reinterpret_cast<u32x4*>(X + row(tid, i) * LD + col(tid)) = ok ? x[i] : u32x4{0, 0, 0, 0};
     }
 };
 
+// The key side of a workgroup that owns rows: its share of the keys, and tiles of k and v on their way into LDS.
+template <typename T, int D, int THREADS>
+struct KeyStream {
+    typedef Stager<T, D, THREADS> St;
+    St k, v;
+    const char *kb, *vb;
+    const unsigned char* mb;  // the mask's row, or any readable byte when there is none
+    long long ks, vs;         // bytes from key to key
+    unsigned k0, v0, kc, vc;  // this thread's first row and column in bytes
+    unsigned live1, live2;    // which keys of the last two tiles of k take part
+    int begin, end, nk, ktile, mstep, open;
+    unsigned char raw;
+
+    __device__ __forceinline__ void init(const DaArgs& a, int tid, int bi, int kh, int part, int last_row) {
+        constexpr int E = (int)sizeof(T);
+        kb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + bi * a.k_sb + kh * a.k_sh);
+        vb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + bi * a.v_sb + kh * a.v_sh);
+        open = a.mask == nullptr;
+        mb = open ? reinterpret_cast<const unsigned char*>(kb) : a.mask + (size_t)bi * a.nk;
+        mstep = open ? 0 : 1;
+        ks = a.k_sn * E;
+        vs = a.v_sn * E;
+        const int c = St::col(tid), r = St::row(tid, 0);
+        k0 = r * (unsigned)ks;
+        v0 = r * (unsigned)vs;
+        kc = (c >= D ? (unsigned)a.k_sm + c - D : c) * E;
+        vc = c * E;
+        nk = a.nk;
+        begin = part * a.span;
+        end = min(min(a.nk, begin + a.span), da_limit(a, last_row));
+        live1 = live2 = 0;
+    }
+    __device__ __forceinline__ int tiles() const { return end > begin ? (end - begin + DA_TILE - 1) / DA_TILE : 0; }
+    // leading tiles of which every row of the workgroup sees all frames (rows see more and more keys: the first row decides)
+    __device__ __forceinline__ int plain(const DaArgs& a, int first_row) const {
+        return a.frame ? max(0, da_limit(a, first_row) - begin) / DA_TILE : tiles();
+    }
+    // vector i of tile t; tiles past the end read the last key again
+    __device__ __forceinline__ void get_k(int tid, int i, int t) {
+        const int key0 = min(begin + t * DA_TILE, nk - 1);
+        k.get(i, kb + key0 * ks, min(k0 + i * St::STEP * (unsigned)ks, min(nk - 1 - key0, DA_TILE) * (unsigned)ks) + kc);
+        if (i == 0) {
+            ktile = begin + t * DA_TILE;
+            raw = mb[(size_t)min(ktile + tid % DA_TILE, nk - 1) * mstep];
+        }
+    }
+    __device__ __forceinline__ void get_v(int i, int t) {
+        const int key0 = min(begin + t * DA_TILE, nk - 1);
+        v.get(i, vb + key0 * vs, min(v0 + i * St::STEP * (unsigned)vs, min(nk - 1 - key0, DA_TILE) * (unsigned)vs) + vc);
+    }
+    __device__ __forceinline__ void put_k(int tid, int i, T* K, float* B) {
+        if (i == 0) {
+            live1 = live2;
+            const bool on = (ktile + tid % DA_TILE < end) & ((open | raw) != 0);
+            live2 = (unsigned)__ballot(on);  // lanes 0..31: the tile's keys
+            B[tid % DA_TILE] = on ? 0.f : -DA_INF;  // the same value from every thread of that key
+        }
+        k.put(tid, i, K, (live2 >> St::row(tid, i)) & 1);
+    }
+    __device__ __forceinline__ void put_v(int tid, int i, T* V, unsigned live) { v.put(tid, i, V, (live >> St::row(tid, i)) & 1); }
+};
+
+// What a tile's scores start from: 0, or -inf for the keys that take no part.
+__device__ __forceinline__ f32x16 da_bias(const float* B, int lh) {
+    f32x16 s;
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+        const f32x4 b = *reinterpret_cast<const f32x4*>(B + 8 * g4 + 4 * lh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g4 + i] = b[i];
+    }
+    return s;
+}
+
+// Which row of the problem a lane of a row-owning workgroup stands for.
+struct RowOf {
+    int bi, kh, part, block0, row0, row, head, qi;
+    bool live;
+    __device__ __forceinline__ RowOf(const DaArgs& a, int wn, int wave, int l31) {
+        const int tile = blockIdx.x % a.tiles;
+        const int rest = blockIdx.x / a.tiles;
+        part = rest % a.parts;
+        bi = rest / a.parts / a.hk;
+        kh = rest / a.parts % a.hk;
+        block0 = tile * 32 * wn;
+        row0 = block0 + wave * 32;
+        live = row0 + l31 < a.rows;
+        row = min(row0 + l31, a.rows - 1);  // rows past the end repeat the last one and are not stored
+        head = kh * a.g + row % a.g;
+        qi = row / a.g;
+    }
+    __device__ __forceinline__ int last(const DaArgs& a, int wn) const { return min(block0 + 32 * wn, a.rows) - 1; }
+};
+
+#define DA_BOOL(x) std::integral_constant<bool, x>()
+
 // ---------------------------------------------------------------------------------------------------------- forward
+// Software pipeline.  A: the scores of tile t + 1 on the matrix unit, tile t's weights 2^(c S - m) on the vector unit; B: tile
+// t's weights times v, and the maximum of tile t + 1.  One barrier per tile, between A and B; the operands that follow it were
+// read before it.  k of tile t + 2 is put into LDS in A (its buffer was last read in the A before), v of tile t + 1 in B.
 template <typename T, int D, int WN>
-__global__ __launch_bounds__(64 * WN, WN == 1 ? 1 : 2) void da_fwd_kernel(const DaArgs a) {
+__global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_kernel(const DaArgs a) {
     typedef Mx<T> M;
+    typedef typename M::Frag Frag;
     typedef Stager<T, D, 64 * WN> St;
     constexpr int W = 2 * D, LD = St::LD, KC = D / 16, CB = W / 32;
     __shared__ __attribute__((aligned(16))) T Ks[2][DA_TILE * LD];
@@ -210,228 +332,304 @@ __global__ __launch_bounds__(64 * WN, WN == 1 ? 1 : 2) void da_fwd_kernel(const 
     __shared__ __attribute__((aligned(16))) float Kb[2][DA_TILE];  // 0, or -inf for keys that take no part
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lh = lane >> 5;
-    const int tile = blockIdx.x % a.tiles;
-    const int rest = blockIdx.x / a.tiles;
-    const int part = rest % a.parts, bh = rest / a.parts;
-    const int bi = bh / a.hk, kh = bh % a.hk;
-    const int block0 = tile * 32 * WN;
-    const int row0 = block0 + wave * 32;
-    const int row = min(row0 + l31, a.rows - 1);  // rows past the end repeat the last one and are not stored
-    const int head = kh * a.g + row % a.g, qi = row / a.g;
-
-    const T* qrow = reinterpret_cast<const T*>(a.q) + bi * a.q_sb + qi * a.q_sn + head * a.q_sh;
-    typename M::Frag q1[KC], q2[KC];
+    const RowOf ro(a, WN, wave, l31);
+    const T* qrow = reinterpret_cast<const T*>(a.q) + ro.bi * a.q_sb + ro.qi * a.q_sn + ro.head * a.q_sh;
+    Frag q1[KC], q2[KC];
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
         q1[i] = M::row(qrow + 16 * i, lh);
         q2[i] = M::row(qrow + a.q_sm + 16 * i, lh);
     }
-    const int lim = da_limit(a, row);
-    const int lim_min = __shfl(lim, 0, 64);  // limits grow with the row
-    const int key_begin = part * a.span;
-    const int key_end = min(min(a.nk, key_begin + a.span), da_limit(a, min(block0 + 32 * WN, a.rows) - 1));
-    const T* kb = reinterpret_cast<const T*>(a.k) + bi * a.k_sb + kh * a.k_sh;
-    const T* vb = reinterpret_cast<const T*>(a.v) + bi * a.v_sb + kh * a.v_sh;
-    const unsigned char* mb = a.mask ? a.mask + (size_t)bi * a.nk : nullptr;
+    const int lim = da_limit(a, ro.row);
+    KeyStream<T, D, 64 * WN> ks;
+    ks.init(a, tid, ro.bi, ro.kh, ro.part, ro.last(a, WN));
+    const int ntiles = ks.tiles(), nplain = ks.plain(a, min(ro.block0, a.rows - 1));
 
-    St st;
-    float rb = 0.f;
-    auto load_tile = [&](int key0) {
-        st.load(
-            tid,
-            [&](int r, int c, bool& ok) {
-                const int key = min(key0 + r, a.nk - 1);
-                ok = key0 + r < key_end && (!mb || mb[key]);
-                return kb + key * a.k_sn + (c >= D ? a.k_sm + c - D : c);
-            },
-            [&](int r, int c) { return vb + min(key0 + r, a.nk - 1) * a.v_sn + c; });
-        if (tid < DA_TILE) rb = key0 + tid < key_end && (!mb || mb[key0 + tid]) ? 0.f : -DA_INF;
-    };
-    auto store_tile = [&](int buf) {
-        st.store(tid, Ks[buf], Vs[buf]);
-        if (tid < DA_TILE) Kb[buf][tid] = rb;
-    };
-
-    f32x16 o1[CB], o2[CB];
+    f32x16 o1[CB], o2[CB], s1, s2, n1, n2;
 #pragma unroll
     for (int j = 0; j < CB; ++j) o1[j] = o2[j] = zero16();
-    float m1 = -DA_INF, m2 = -DA_INF, l1 = 0.f, l2 = 0.f;
+    float m1 = -DA_INF, m2 = -DA_INF, l1 = 0.f, l2 = 0.f, x1 = -DA_INF, x2 = -DA_INF;
+    Frag ga, gb;  // the first operands of the next A
 
-    // scores -> weights 2^(c S - m), running maximum m of every lane's row (both lane halves hold the same one).  The
-    // accumulators are rescaled only when the maximum has grown by more than 2^8: weights stay below 256.
-    auto softmax = [&](f32x16& s, float& m, float& l, f32x16* o, int cur, int key0) {
-        if (mb || key0 + DA_TILE > key_end) {
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4) {
-                const f32x4 kbias = *reinterpret_cast<const f32x4*>(&Kb[cur][8 * g4 + 4 * lh]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[4 * g4 + e] += kbias[e];
-            }
+    // one entry of both maps' scores of the tile at key0: later frames to -inf (EDGE), running maximum
+    auto entry = [&](auto edge, f32x16& u, f32x16& w, int r, int key0) {
+        if (decltype(edge)::value) {
+            const bool hide = key0 + acc_index(r, lh) >= lim;
+            u[r] = hide ? -DA_INF : u[r];
+            w[r] = hide ? -DA_INF : w[r];
         }
-        if (key0 + DA_TILE > lim_min) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (key0 + acc_index(r, lh) >= lim) s[r] = -DA_INF;
-        }
-        float mx = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.c;
-        if (__any(mx > m + 8.f)) {
-            const float mn = fmaxf(m, mx);
-            const float f = m == -DA_INF ? 0.f : exp2f(m - mn);
-            m = mn;
-            l *= f;
+        x1 = fmaxf(x1, u[r]);
+        x2 = fmaxf(x2, w[r]);
+    };
+    auto finish_max = [&]() {  // over both lane halves, in the exponent's units
+        x1 = half_max(x1) * a.c;
+        x2 = half_max(x2) * a.c;
+    };
+    auto ready = [&](int buf) {  // what the next A starts from
+        n1 = n2 = da_bias(Kb[buf], lh);
+        ga = M::row(Ks[buf] + l31 * LD, lh);
+        gb = M::row(Ks[buf] + l31 * LD + D, lh);
+    };
+    auto body = [&](auto next, auto edge, int t) {
+        constexpr bool NEXT = decltype(next)::value;
+        const int cur = t & 1, nxt = cur ^ 1, key1 = ks.begin + (t + 1) * DA_TILE;
+        // The sums are rescaled only when a maximum has grown by more than 2^8: weights stay below 256.
+        if (__any(x1 > m1 + 8.f || x2 > m2 + 8.f)) {
+            const float a1 = fmaxf(m1, x1), a2 = fmaxf(m2, x2);
+            const float f1 = m1 == -DA_INF ? 0.f : exp2f(m1 - a1), f2 = m2 == -DA_INF ? 0.f : exp2f(m2 - a2);
+            m1 = a1;
+            m2 = a2;
+            l1 *= f1;
+            l2 *= f2;
 #pragma unroll
             for (int j = 0; j < CB; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[j][r] *= f;
+                for (int r = 0; r < 16; ++r) {
+                    o1[j][r] *= f1;
+                    o2[j][r] *= f2;
+                }
         }
-        const float mu = m == -DA_INF ? 0.f : m;
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -mu));
-            sum += s[r];
-        }
-        l += sum;
-    };
-
-    const int ntiles = key_end > key_begin ? (key_end - key_begin + DA_TILE - 1) / DA_TILE : 0;
-    if (ntiles > 0) {
-        load_tile(key_begin);
-        store_tile(0);
-        if (ntiles > 1) load_tile(key_begin + DA_TILE);
-    }
-    __syncthreads();
-    for (int t = 0; t < ntiles; ++t) {
-        const int cur = t & 1, key0 = key_begin + t * DA_TILE;
-        const T* Kc = Ks[cur] + l31 * LD;
-        f32x16 s1 = zero16(), s2 = zero16();
+        const float u1 = m1 == -DA_INF ? 0.f : m1, u2 = m2 == -DA_INF ? 0.f : m2;
+        const T* Kn = Ks[nxt] + l31 * LD;
+        constexpr int SL = KC * M::STEPS;
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
-            M::mma(s1, M::row(Kc + 16 * i, lh), q1[i]);
-            M::mma(s2, M::row(Kc + D + 16 * i, lh), q2[i]);
-        }
-        if (t + 1 < ntiles) {  // tile t+1 has been in flight since the last trip; its buffer's readers passed the barrier
-            store_tile(cur ^ 1);
-            if (t + 2 < ntiles) load_tile(key0 + 2 * DA_TILE);
-        }
-        softmax(s1, m1, l1, o1, cur, key0);
-        softmax(s2, m2, l2, o2, cur, key0);
+            const Frag fa = ga, fb = gb;
+            if (NEXT && i + 1 < KC) {
+                ga = M::row(Kn + 16 * (i + 1), lh);
+                gb = M::row(Kn + D + 16 * (i + 1), lh);
+            }
 #pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2) {
-            const typename M::Frag p1 = M::reg(s1, t2), p2 = M::reg(s2, t2);
+            for (int e = 0; e < M::STEPS; ++e) {
+                if (NEXT) {
+                    M::step(n1, fa, q1[i], e);
+                    M::step(n2, fb, q2[i], e);
+                }
+                const int slot = i * M::STEPS + e;
 #pragma unroll
-            for (int j = 0; j < CB; ++j) {
-                const typename M::Frag vf = M::col(Vs[cur], LD, 16 * t2, 32 * j, lane);
-                M::mma(o1[j], vf, p1);
-                M::mma(o2[j], vf, p2);
+                for (int it = slot * 32 / SL; it < (slot + 1) * 32 / SL; ++it) {
+                    const int r = it >> 1;
+                    if (it & 1) {
+                        s2[r] = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -u2));
+                        l2 += s2[r];
+                    } else {
+                        s1[r] = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -u1));
+                        l1 += s1[r];
+                    }
+                }
+                if (NEXT) {
+#pragma unroll
+                    for (int f = slot * St::F / SL; f < (slot + 1) * St::F / SL; ++f) {
+                        ks.put_k(tid, f, Ks[cur], Kb[cur]);
+                        ks.get_k(tid, f, t + 3);
+                    }
+                }
+                da_pin();
             }
         }
+        Frag vn = M::col(Vs[cur], LD, 0, 0, lane);
         __syncthreads();
+        da_pin();
+        x1 = x2 = -DA_INF;
+        constexpr int SB = 2 * CB * M::RSTEPS, S0 = SB >= 16 ? 2 : 0;  // the scores' last products are still in flight
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+            const typename M::RegFrag p1 = M::reg(s1, t2), p2 = M::reg(s2, t2);
+#pragma unroll
+            for (int j = 0; j < CB; ++j) {
+                const Frag vf = vn;
+                if (t2 * CB + j + 1 < 2 * CB) vn = M::col(Vs[cur], LD, 16 * ((t2 * CB + j + 1) / CB), 32 * ((j + 1) % CB), lane);
+#pragma unroll
+                for (int e = 0; e < M::RSTEPS; ++e) {
+                    M::rstep(o1[j], vf, p1, e);
+                    M::rstep(o2[j], vf, p2, e);
+                    const int slot = (t2 * CB + j) * M::RSTEPS + e;
+                    if (NEXT && slot >= S0) {
+#pragma unroll
+                        for (int r = (slot - S0) * 16 / (SB - S0); r < (slot - S0 + 1) * 16 / (SB - S0); ++r) entry(edge, n1, n2, r, key1);
+                    }
+                    if (NEXT) {
+#pragma unroll
+                        for (int f = slot * St::F / SB; f < (slot + 1) * St::F / SB; ++f) {
+                            ks.put_v(tid, f, Vs[nxt], ks.live1);
+                            ks.get_v(f, t + 2);
+                        }
+                    }
+                    da_pin();
+                }
+            }
+        }
+        if (NEXT) {
+            s1 = n1;
+            s2 = n2;
+            finish_max();
+            ready(cur);
+        }
+    };
+
+    if (ntiles > 0) {
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            ks.get_k(tid, f, 0);
+            ks.get_v(f, 0);
+        }
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            ks.put_k(tid, f, Ks[0], Kb[0]);
+            ks.put_v(tid, f, Vs[0], ks.live2);
+            ks.get_v(f, 1);
+        }
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) ks.get_k(tid, f, 1);
+        __syncthreads();
+        s1 = s2 = da_bias(Kb[0], lh);
+        const T* K0 = Ks[0] + l31 * LD;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            const Frag fa = M::row(K0 + 16 * i, lh), fb = M::row(K0 + D + 16 * i, lh);
+#pragma unroll
+            for (int e = 0; e < M::STEPS; ++e) {
+                M::step(s1, fa, q1[i], e);
+                M::step(s2, fb, q2[i], e);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) entry(DA_BOOL(true), s1, s2, r, ks.begin);
+        finish_max();
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            ks.put_k(tid, f, Ks[1], Kb[1]);
+            ks.get_k(tid, f, 2);
+        }
+        __syncthreads();
+        ready(1);
+        int t = 0;
+        if (M::ONE_LOOP) {
+            for (; t < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+        } else {  // tiles that every row of the workgroup sees whole come first
+            for (; t + 1 < min(nplain, ntiles); ++t) body(DA_BOOL(true), DA_BOOL(false), t);
+            for (; t + 1 < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+            body(DA_BOOL(false), DA_BOOL(false), t);
+        }
     }
     l1 += __shfl_xor(l1, 32, 64);
     l2 += __shfl_xor(l2, 32, 64);
-    if (row0 + l31 >= a.rows) return;
+    if (!ro.live) return;
+    const size_t e = ((size_t)ro.bi * a.hk + ro.kh) * a.rows + ro.row, n = (size_t)a.b * a.hk * a.rows;
     if (a.parts > 1) {  // unnormalised sums with their maximum, joined by da_join_kernel
-        const size_t e = ((size_t)part * a.b * a.hk + bh) * a.rows + row;
-        float* po = a.part + e * 2 * W;
+        float* po = a.part + (ro.part * n + e) * 2 * W;
 #pragma unroll
         for (int j = 0; j < CB; ++j)
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int ch = 32 * j + 8 * g4 + 4 * lh;
-                f32x4 x, y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = o1[j][4 * g4 + i];
-                    y[i] = o2[j][4 * g4 + i];
-                }
-                *reinterpret_cast<f32x4*>(po + ch) = x;
-                *reinterpret_cast<f32x4*>(po + W + ch) = y;
+                *reinterpret_cast<f32x4*>(po + ch) = quad(o1[j], g4);
+                *reinterpret_cast<f32x4*>(po + W + ch) = quad(o2[j], g4);
             }
-        if (lh == 0) *reinterpret_cast<f32x4*>(a.ml + e * 4) = f32x4{m1, l1, m2, l2};
+        if (lh == 0) *reinterpret_cast<f32x4*>(a.ml + (ro.part * n + e) * 4) = f32x4{m1, l1, m2, l2};
         return;
     }
-    const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : 1.f / l2, lam = da_lambda(a, head);
-    T* out = reinterpret_cast<T*>(a.out) + (((size_t)bi * a.nq + qi) * a.h + head) * W;
-    T* out2 = a.o2 ? reinterpret_cast<T*>(a.o2) + (((size_t)bi * a.nq + qi) * a.h + head) * W : nullptr;
+    const float i1 = l1 == 0.f ? 0.f : 1.f / l1, i2 = l2 == 0.f ? 0.f : 1.f / l2, lam = da_lambda(a, ro.head);
+    const size_t o = (((size_t)ro.bi * a.nq + ro.qi) * a.h + ro.head) * W;
+    T* out = reinterpret_cast<T*>(a.out) + o;
 #pragma unroll
     for (int j = 0; j < CB; ++j)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
             const int ch = 32 * j + 8 * g4 + 4 * lh;
-            f32x4 x, y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                y[i] = o2[j][4 * g4 + i] * i2;
-                x[i] = o1[j][4 * g4 + i] * i1 - lam * y[i];
+            const f32x4 x = quad(o1[j], g4) * i1, y = quad(o2[j], g4) * i2;
+            M::store4(out + ch, x - y * lam);
+            if (a.maps) {
+                *reinterpret_cast<f32x4*>(a.maps + 2 * o + ch) = x;
+                *reinterpret_cast<f32x4*>(a.maps + 2 * o + W + ch) = y;
             }
-            M::store4(out + ch, x);
-            if (out2) M::store4(out2 + ch, y);
         }
     if (a.lse && lh == 0) {
-        const size_t e = (size_t)bh * a.rows + row, n = (size_t)a.b * a.hk * a.rows;
         a.lse[e] = l1 == 0.f ? DA_INF : m1 + log2f(l1);
         a.lse[n + e] = l2 == 0.f ? DA_INF : m2 + log2f(l2);
     }
 }
 
-// Joins the parts of a row: one workgroup per row, W / 4 threads across the channels, the rest across the parts.
+// Joins the parts of a row.  Up to 32 parts: W / 4 threads per row, each goes over the parts by itself (every thread of a row
+// reads the same maxima and sums of weights, from the cache).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
+    constexpr int W = 2 * D, CT = W / 4;
+    const size_t n = (size_t)a.b * a.hk * a.rows, e = (size_t)blockIdx.x * (256 / CT) + threadIdx.x / CT;
+    if (e >= n) return;
+    const int ch = 4 * (threadIdx.x % CT);
+    const int bh = (int)(e / a.rows), row = (int)(e % a.rows);
+    const int head = (bh % a.hk) * a.g + row % a.g;
+    float M1 = -DA_INF, M2 = -DA_INF, L1 = 0.f, L2 = 0.f;
+    for (int p = 0; p < a.parts; ++p) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ml + (p * n + e) * 4);
+        M1 = fmaxf(M1, v[0]);
+        M2 = fmaxf(M2, v[2]);
+    }
+    const float u1 = M1 == -DA_INF ? 0.f : M1, u2 = M2 == -DA_INF ? 0.f : M2;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 4
+    for (int p = 0; p < a.parts; ++p) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ml + (p * n + e) * 4);
+        const float* s = a.part + (p * n + e) * 2 * W + ch;
+        const float w1 = exp2f(v[0] - u1), w2 = exp2f(v[2] - u2);
+        x += *reinterpret_cast<const f32x4*>(s) * w1;
+        y += *reinterpret_cast<const f32x4*>(s + W) * w2;
+        L1 = fmaf(v[1], w1, L1);
+        L2 = fmaf(v[3], w2, L2);
+    }
+    x *= L1 == 0.f ? 0.f : 1.f / L1;
+    y *= L2 == 0.f ? 0.f : 1.f / L2;
+    const size_t o = (((size_t)(bh / a.hk) * a.nq + row / a.g) * a.h + head) * W + ch;
+    Mx<T>::store4(reinterpret_cast<T*>(a.out) + o, x - y * da_lambda(a, head));
+    if (a.maps) {
+        *reinterpret_cast<f32x4*>(a.maps + 2 * (o - ch) + ch) = x;
+        *reinterpret_cast<f32x4*>(a.maps + 2 * (o - ch) + W + ch) = y;
+    }
+    if (a.lse && ch == 0) {
+        a.lse[e] = L1 == 0.f ? DA_INF : u1 + log2f(L1);
+        a.lse[n + e] = L2 == 0.f ? DA_INF : u2 + log2f(L2);
+    }
+}
+
+// More parts (few rows, a long axis): one workgroup per row, the parts dealt out over its threads, sums in a fixed tree.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void da_join_row_kernel(const DaArgs a) {
     constexpr int W = 2 * D, CT = 2 * W / 4, PT = 256 / CT;  // CT threads hold one part's two sums
-    __shared__ float red[4][256];
+    __shared__ float red[4][4];
     __shared__ f32x4 sum[256];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, wave = tid >> 6;
     const size_t n = (size_t)a.b * a.hk * a.rows, e = blockIdx.x;
     const int bh = (int)(e / a.rows), row = (int)(e % a.rows);
     const int head = (bh % a.hk) * a.g + row % a.g;
-    float M[2] = {-DA_INF, -DA_INF}, L[2] = {0.f, 0.f};
-    for (int p = tid; p < a.parts; p += 256) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ml + (p * n + e) * 4);
-        M[0] = fmaxf(M[0], v[0]);
-        M[1] = fmaxf(M[1], v[2]);
+    const f32x4 none = {-DA_INF, 0.f, -DA_INF, 0.f};
+    const f32x4 mine = tid < a.parts ? *reinterpret_cast<const f32x4*>(a.ml + (tid * n + e) * 4) : none;  // at most 256 parts
+    float u[2], L[2];
+    const float w1 = wave_max(mine[0]), w2 = wave_max(mine[2]);
+    if ((tid & 63) == 0) {
+        red[0][wave] = w1;
+        red[1][wave] = w2;
     }
-    red[0][tid] = M[0];
-    red[1][tid] = M[1];
     __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-        if (tid < h) {
-            red[0][tid] = fmaxf(red[0][tid], red[0][tid + h]);
-            red[1][tid] = fmaxf(red[1][tid], red[1][tid + h]);
-        }
-        __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        u[m] = fmaxf(fmaxf(red[m][0], red[m][1]), fmaxf(red[m][2], red[m][3]));
+        if (u[m] == -DA_INF) u[m] = 0.f;
     }
-    M[0] = red[0][0] == -DA_INF ? 0.f : red[0][0];
-    M[1] = red[1][0] == -DA_INF ? 0.f : red[1][0];
-    for (int p = tid; p < a.parts; p += 256) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ml + (p * n + e) * 4);
-        L[0] += v[1] * exp2f(v[0] - M[0]);
-        L[1] += v[3] * exp2f(v[2] - M[1]);
+    const float s1 = wave_sum(mine[1] * exp2f(mine[0] - u[0])), s2 = wave_sum(mine[3] * exp2f(mine[2] - u[1]));
+    if ((tid & 63) == 0) {
+        red[2][wave] = s1;
+        red[3][wave] = s2;
     }
-    red[2][tid] = L[0];
-    red[3][tid] = L[1];
-    __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-        if (tid < h) {
-            red[2][tid] += red[2][tid + h];
-            red[3][tid] += red[3][tid + h];
-        }
-        __syncthreads();
-    }
-    L[0] = red[2][0];
-    L[1] = red[3][0];
     const int ch = tid % CT, map = ch >= CT / 2 ? 1 : 0;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int p = tid / CT; p < a.parts; p += PT) {
-        const float w = exp2f(a.ml[(p * n + e) * 4 + 2 * map] - M[map]);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + (p * n + e) * 2 * W + 4 * ch);
-        if (w != 0.f) acc += v * w;
-    }
+#pragma unroll 4
+    for (int p = tid / CT; p < a.parts; p += PT)
+        acc += *reinterpret_cast<const f32x4*>(a.part + (p * n + e) * 2 * W + 4 * ch) * exp2f(a.ml[(p * n + e) * 4 + 2 * map] - u[map]);
     sum[tid] = acc;
     __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 2; ++m) L[m] = (red[2 + m][0] + red[2 + m][1]) + (red[2 + m][2] + red[2 + m][3]);
     if (tid < CT / 2) {
         f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
         for (int p = 0; p < PT; ++p) {
@@ -440,20 +638,22 @@ __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
         }
         x *= L[0] == 0.f ? 0.f : 1.f / L[0];
         y *= L[1] == 0.f ? 0.f : 1.f / L[1];
-        const size_t o = (((size_t)(bh / a.hk) * a.nq + row / a.g) * a.h + head) * W + 4 * tid;
-        if (a.o2) Mx<T>::store4(reinterpret_cast<T*>(a.o2) + o, y);
-        x -= y * da_lambda(a, head);
-        Mx<T>::store4(reinterpret_cast<T*>(a.out) + o, x);
+        const size_t o = (((size_t)(bh / a.hk) * a.nq + row / a.g) * a.h + head) * W;
+        Mx<T>::store4(reinterpret_cast<T*>(a.out) + o + 4 * tid, x - y * da_lambda(a, head));
+        if (a.maps) {
+            *reinterpret_cast<f32x4*>(a.maps + 2 * o + 4 * tid) = x;
+            *reinterpret_cast<f32x4*>(a.maps + 2 * o + W + 4 * tid) = y;
+        }
     }
-    if (a.lse && tid < 2) a.lse[tid * n + e] = L[tid] == 0.f ? DA_INF : M[tid] + log2f(L[tid]);
+    if (a.lse && tid < 2) a.lse[tid * n + e] = L[tid] == 0.f ? DA_INF : u[tid] + log2f(L[tid]);
 }
 
 // --------------------------------------------------------------------------------------------------------- backward
-// D_1, D_2 of every row, and partial sums of D_2 per head: a workgroup owns 256 / LPR rows per trip of one (batch, head)
+// The constants of every row for the backward pass (D_1, D_2 among them), and partial sums of D_2 per head: a workgroup owns 256 / LPR rows per trip of one (batch, head)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void da_delta_kernel(const DaArgs a) {
     constexpr int W = 2 * D, V = 4, LPR = W / V;
-    __shared__ double red[256];
+    __shared__ double red[4];
     const int chunk = blockIdx.x % a.lchunks, bh = blockIdx.x / a.lchunks;
     const int bi = bh / a.h, head = bh % a.h;
     const int kh = head / a.g, g = head % a.g;
@@ -462,214 +662,258 @@ __global__ __launch_bounds__(256) void da_delta_kernel(const DaArgs a) {
     const size_t n = (size_t)a.b * a.hk * a.rows;
     double total = 0.0;
     for (int q = chunk * (256 / LPR) + threadIdx.x / LPR; q < a.nq; q += a.lchunks * (256 / LPR)) {
-        const size_t o = (((size_t)bi * a.nq + q) * a.h + head) * W + V * sub;
-        float go[V], ou[V], o2[V];
-        Vec<T, V>::load(reinterpret_cast<const T*>(a.go) + o, go);
-        Vec<T, V>::load(reinterpret_cast<const T*>(a.out) + o, ou);
-        Vec<T, V>::load(reinterpret_cast<const T*>(a.o2) + o, o2);
+        const size_t o = (((size_t)bi * a.nq + q) * a.h + head) * W;
+        float go[V];
+        Vec<T, V>::load(reinterpret_cast<const T*>(a.go) + o + V * sub, go);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.maps + 2 * o + V * sub);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(a.maps + 2 * o + W + V * sub);
         float d1 = 0.f, d2 = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            d2 = fmaf(go[i], o2[i], d2);
-            d1 = fmaf(go[i], fmaf(lam, o2[i], ou[i]), d1);
+            d1 = fmaf(go[i], x[i], d1);
+            d2 = fmaf(go[i], y[i], d2);
         }
         for (int s = LPR / 2; s > 0; s >>= 1) {
             d1 += __shfl_xor(d1, s, 64);
             d2 += __shfl_xor(d2, s, 64);
         }
         if (sub == 0) {
-            const size_t e = ((size_t)bi * a.hk + kh) * a.rows + (size_t)q * a.g + g;
-            a.delta[e] = d1;
-            a.delta[n + e] = d2;
+            const int row = q * a.g + g;
+            const size_t e = ((size_t)bi * a.hk + kh) * a.rows + row;
+            a.stat[e] = a.lse[e];
+            a.stat[n + e] = a.lse[n + e];
+            a.stat[2 * n + e] = d1;
+            a.stat[3 * n + e] = d2;
+            a.stat[4 * n + e] = lam;
+            a.stat[5 * n + e] = __int_as_float(da_limit(a, row));
             total += (double)d2;
         }
     }
-    red[threadIdx.x] = total;
+    total = wave_sum_d(total);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = total;
     __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-        if ((int)threadIdx.x < h) red[threadIdx.x] += red[threadIdx.x + h];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) a.lpart[(size_t)bh * a.lchunks + chunk] = red[0];
+    if (threadIdx.x == 0) a.lpart[(size_t)bh * a.lchunks + chunk] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // dlam[h] = - sum over batch and chunks: one workgroup per head
 __global__ __launch_bounds__(256) void da_dlam_kernel(const DaArgs a) {
-    __shared__ double red[256];
+    __shared__ double red[4];
     const int head = blockIdx.x, n = a.b * a.lchunks;
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += 256)
         s += a.lpart[((size_t)(i / a.lchunks) * a.h + head) * a.lchunks + i % a.lchunks];
-    red[threadIdx.x] = s;
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-        if ((int)threadIdx.x < h) red[threadIdx.x] += red[threadIdx.x + h];
-        __syncthreads();
-    }
     if (threadIdx.x == 0) {
+        const float r = (float)-((red[0] + red[1]) + (red[2] + red[3]));
         if (a.lam_bf16)
-            reinterpret_cast<bf16_t*>(a.dlam)[head] = (bf16_t)(float)-red[0];
+            reinterpret_cast<bf16_t*>(a.dlam)[head] = (bf16_t)r;
         else
-            reinterpret_cast<float*>(a.dlam)[head] = (float)-red[0];
+            reinterpret_cast<float*>(a.dlam)[head] = r;
     }
 }
 
-// dq: a wave owns 32 rows (everything about them is one value per lane) and streams key tiles.
+// dq: a wave owns 32 rows (everything about them is one value per lane) and streams key tiles.  A: S and dP of tile t + 1, dS of
+// tile t; B: dq += dS k of tile t.  One barrier per tile, between A and B.  k: two tiles in use, one being put, and one that a
+// slower wave may still be reading: four buffers; v is read in A only: two.
 template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void da_dq_kernel(const DaArgs a) {
+__global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArgs a) {
     typedef Mx<T> M;
+    typedef typename M::Frag Frag;
     typedef Stager<T, D, 256> St;
-    constexpr int W = 2 * D, LD = St::LD, KC = D / 16, VC = W / 16, DB = (D + 31) / 32;
-    constexpr int LDT = LD;
-    __shared__ __attribute__((aligned(16))) T Ks[2][DA_TILE * LD];
+    constexpr int W = 2 * D, LD = St::LD, KC = D / 16, DB = (D + 31) / 32, C2 = D < 32 ? 0 : D;
+    __shared__ __attribute__((aligned(16))) T Ks[4][DA_TILE * LD];
     __shared__ __attribute__((aligned(16))) T Vs[2][DA_TILE * LD];
-    __shared__ __attribute__((aligned(16))) float Kb[2][DA_TILE];
+    __shared__ __attribute__((aligned(16))) float Kb[4][DA_TILE];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lh = lane >> 5;
-    const int tile = blockIdx.x % a.tiles;
-    const int rest = blockIdx.x / a.tiles;
-    const int part = rest % a.parts, bh = rest / a.parts;
-    const int bi = bh / a.hk, kh = bh % a.hk;
-    const int block0 = tile * 128;
-    const int row0 = block0 + wave * 32;
-    const int row = min(row0 + l31, a.rows - 1);
-    const int head = kh * a.g + row % a.g, qi = row / a.g;
-    const size_t n = (size_t)a.b * a.hk * a.rows, e = (size_t)bh * a.rows + row;
-
-    const T* qrow = reinterpret_cast<const T*>(a.q) + bi * a.q_sb + qi * a.q_sn + head * a.q_sh;
-    const T* grow = reinterpret_cast<const T*>(a.go) + (((size_t)bi * a.nq + qi) * a.h + head) * W;
-    typename M::Frag q1[KC], q2[KC], go[VC];
+    const RowOf ro(a, 4, wave, l31);
+    const size_t n = (size_t)a.b * a.hk * a.rows, e0 = ((size_t)ro.bi * a.hk + ro.kh) * a.rows + ro.row;
+    const size_t o = (((size_t)ro.bi * a.nq + ro.qi) * a.h + ro.head) * W;
+    const T* qrow = reinterpret_cast<const T*>(a.q) + ro.bi * a.q_sb + ro.qi * a.q_sn + ro.head * a.q_sh;
+    const T* grow = reinterpret_cast<const T*>(a.go) + o;
+    Frag q1[KC], q2[KC], go[2 * KC];
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
         q1[i] = M::row(qrow + 16 * i, lh);
         q2[i] = M::row(qrow + a.q_sm + 16 * i, lh);
+        go[2 * i] = M::row(grow + 32 * i, lh);
+        go[2 * i + 1] = M::row(grow + 32 * i + 16, lh);
     }
-#pragma unroll
-    for (int i = 0; i < VC; ++i) go[i] = M::row(grow + 16 * i, lh);
-    const float e1 = a.lse[e], e2 = a.lse[n + e], d1 = a.delta[e], d2 = a.delta[n + e];
-    const int lim = da_limit(a, row);
-    const int lim_min = __shfl(lim, 0, 64);
-    const int key_begin = part * a.span;
-    const int key_end = min(min(a.nk, key_begin + a.span), da_limit(a, min(block0 + 128, a.rows) - 1));
-    const T* kb = reinterpret_cast<const T*>(a.k) + bi * a.k_sb + kh * a.k_sh;
-    const T* vb = reinterpret_cast<const T*>(a.v) + bi * a.v_sb + kh * a.v_sh;
-    const unsigned char* mb = a.mask ? a.mask + (size_t)bi * a.nk : nullptr;
+    const float e1 = a.stat[e0], e2 = a.stat[n + e0], d1 = a.stat[2 * n + e0], d2 = a.stat[3 * n + e0];
+    const int lim = da_limit(a, ro.row);
+    KeyStream<T, D, 256> ks;
+    ks.init(a, tid, ro.bi, ro.kh, ro.part, ro.last(a, 4));
+    const int ntiles = ks.tiles(), nplain = ks.plain(a, min(ro.block0, a.rows - 1));
 
-    St st;
-    float rb = 0.f;
-    auto load_tile = [&](int key0) {
-        st.load(
-            tid,
-            [&](int r, int c, bool& ok) {
-                const int key = min(key0 + r, a.nk - 1);
-                ok = key0 + r < key_end && (!mb || mb[key]);
-                return kb + key * a.k_sn + (c >= D ? a.k_sm + c - D : c);
-            },
-            [&](int r, int c) { return vb + min(key0 + r, a.nk - 1) * a.v_sn + c; });
-        if (tid < DA_TILE) rb = key0 + tid < key_end && (!mb || mb[key0 + tid]) ? 0.f : -DA_INF;
-    };
-    auto store_tile = [&](int buf) {
-        st.store(tid, Ks[buf], Vs[buf]);
-        if (tid < DA_TILE) Kb[buf][tid] = rb;
-    };
-    f32x16 g1[DB], g2[DB];
+    f32x16 g1[DB], g2[DB], s1, s2, dp = zero16(), n1, n2, np;
 #pragma unroll
     for (int j = 0; j < DB; ++j) g1[j] = g2[j] = zero16();
+    Frag ga, gb, gc, gd;  // the first operands of the next A
 
-    const int ntiles = key_end > key_begin ? (key_end - key_begin + DA_TILE - 1) / DA_TILE : 0;
-    if (ntiles > 0) {
-        load_tile(key_begin);
-        store_tile(0);
-        if (ntiles > 1) load_tile(key_begin + DA_TILE);
-    }
-    __syncthreads();
-    for (int t = 0; t < ntiles; ++t) {
-        const int cur = t & 1, key0 = key_begin + t * DA_TILE;
-        const T* Kc = Ks[cur] + l31 * LD;
-        const T* Vc = Vs[cur] + l31 * LD;
-        f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
+    auto ready = [&](int kbuf, int vbuf) {
+        n1 = n2 = da_bias(Kb[kbuf], lh);
+        np = zero16();
+        ga = M::row(Ks[kbuf] + l31 * LD, lh);
+        gb = M::row(Ks[kbuf] + l31 * LD + D, lh);
+        gc = M::row(Vs[vbuf] + l31 * LD, lh);
+        gd = M::row(Vs[vbuf] + l31 * LD + 16, lh);
+    };
+    auto body = [&](auto next, auto edge, int t) {
+        constexpr bool NEXT = decltype(next)::value;
+        const int key0 = ks.begin + t * DA_TILE, b0 = t & 3, b2 = (t + 2) & 3;
+        const T *Kn = Ks[(t + 1) & 3] + l31 * LD, *Vn = Vs[(t + 1) & 1] + l31 * LD;
+        constexpr int SL = KC * M::STEPS;
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
-            M::mma(s1, M::row(Kc + 16 * i, lh), q1[i]);
-            M::mma(s2, M::row(Kc + D + 16 * i, lh), q2[i]);
-        }
+            const Frag fa = ga, fb = gb, fc = gc, fd = gd;
+            if (NEXT && i + 1 < KC) {
+                ga = M::row(Kn + 16 * (i + 1), lh);
+                gb = M::row(Kn + D + 16 * (i + 1), lh);
+                gc = M::row(Vn + 32 * (i + 1), lh);
+                gd = M::row(Vn + 32 * (i + 1) + 16, lh);
+            }
 #pragma unroll
-        for (int i = 0; i < VC; ++i) M::mma(dp, M::row(Vc + 16 * i, lh), go[i]);
-        if (t + 1 < ntiles) {
-            store_tile(cur ^ 1);
-            if (t + 2 < ntiles) load_tile(key0 + 2 * DA_TILE);
-        }
-        if (mb || key0 + DA_TILE > key_end) {
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4) {
-                const f32x4 kbias = *reinterpret_cast<const f32x4*>(&Kb[cur][8 * g4 + 4 * lh]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s1[4 * g4 + i] += kbias[i];
-                    s2[4 * g4 + i] += kbias[i];
+            for (int e = 0; e < M::STEPS; ++e) {
+                if (NEXT) {
+                    M::step(n1, fa, q1[i], e);
+                    M::step(np, fc, go[2 * i], e);
+                    M::step(n2, fb, q2[i], e);
+                    M::step(np, fd, go[2 * i + 1], e);
                 }
+                const int slot = i * M::STEPS + e;
+#pragma unroll
+                for (int it = slot * 32 / SL; it < (slot + 1) * 32 / SL; ++it) {
+                    const int r = it >> 1;
+                    f32x16& s = it & 1 ? s2 : s1;
+                    if (decltype(edge)::value) s[r] = key0 + acc_index(r, lh) >= lim ? -DA_INF : s[r];
+                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, it & 1 ? -e2 : -e1)) * (dp[r] - (it & 1 ? d2 : d1));
+                }
+                if (NEXT) {
+#pragma unroll
+                    for (int f = slot * St::F / SL; f < (slot + 1) * St::F / SL; ++f) {
+                        ks.put_k(tid, f, Ks[b2], Kb[b2]);
+                        ks.put_v(tid, f, Vs[t & 1], ks.live2);
+                        ks.get_k(tid, f, t + 3);
+                        ks.get_v(f, t + 3);
+                    }
+                }
+                da_pin();
             }
         }
-        if (key0 + DA_TILE > lim_min) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (key0 + acc_index(r, lh) >= lim) s1[r] = s2[r] = -DA_INF;
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s1[r] = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -e1)) * (dp[r] - d1);
-            s2[r] = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -e2)) * (dp[r] - d2);
-        }
+        Frag k1 = M::col(Ks[b0], LD, 0, 0, lane), k2 = M::col(Ks[b0], LD, 0, C2, lane);
+        __syncthreads();
+        da_pin();
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
-            const typename M::Frag p1 = M::reg(s1, t2), p2 = M::reg(s2, t2);
+            const typename M::RegFrag p1 = M::reg(s1, t2), p2 = M::reg(s2, t2);
 #pragma unroll
             for (int j = 0; j < DB; ++j) {
-                // D = 16: the upper 16 columns of the fragment belong to the other map (or the padding) and are not stored
-                M::mma(g1[j], M::col(Ks[cur], LDT, 16 * t2, 32 * j, lane), p1);
-                M::mma(g2[j], M::col(Ks[cur], LDT, 16 * t2, (D < 32 ? 0 : D) + 32 * j, lane), p2);
+                const Frag c1 = k1, c2 = k2;
+                if (t2 * DB + j + 1 < 2 * DB) {
+                    k1 = M::col(Ks[b0], LD, 16 * ((t2 * DB + j + 1) / DB), 32 * ((j + 1) % DB), lane);
+                    k2 = M::col(Ks[b0], LD, 16 * ((t2 * DB + j + 1) / DB), C2 + 32 * ((j + 1) % DB), lane);
+                }
+                // D = 16: each product holds 16 columns of the other map's keys too; they are not stored
+#pragma unroll
+                for (int e = 0; e < M::RSTEPS; ++e) {
+                    M::rstep(g1[j], c1, p1, e);
+                    M::rstep(g2[j], c2, p2, e);
+                }
+                da_pin();
             }
         }
+        if (NEXT) {
+            s1 = n1;
+            s2 = n2;
+            dp = np;
+            ready(b2, t & 1);
+        }
+    };
+
+    if (ntiles > 0) {
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            ks.get_k(tid, f, 0);
+            ks.get_v(f, 0);
+        }
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            ks.put_k(tid, f, Ks[0], Kb[0]);
+            ks.put_v(tid, f, Vs[0], ks.live2);
+        }
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            ks.get_k(tid, f, 1);
+            ks.get_v(f, 1);
+        }
         __syncthreads();
+        s1 = s2 = da_bias(Kb[0], lh);
+        const T *K0 = Ks[0] + l31 * LD, *V0 = Vs[0] + l31 * LD;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            const Frag fa = M::row(K0 + 16 * i, lh), fb = M::row(K0 + D + 16 * i, lh);
+            const Frag fc = M::row(V0 + 32 * i, lh), fd = M::row(V0 + 32 * i + 16, lh);
+#pragma unroll
+            for (int e = 0; e < M::STEPS; ++e) {
+                M::step(s1, fa, q1[i], e);
+                M::step(dp, fc, go[2 * i], e);
+                M::step(s2, fb, q2[i], e);
+                M::step(dp, fd, go[2 * i + 1], e);
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            ks.put_k(tid, f, Ks[1], Kb[1]);
+            ks.put_v(tid, f, Vs[1], ks.live2);
+            ks.get_k(tid, f, 2);
+            ks.get_v(f, 2);
+        }
+        __syncthreads();
+        ready(1, 1);
+        int t = 0;
+        if (M::ONE_LOOP) {
+            for (; t < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+        } else {
+            for (; t < min(nplain, ntiles - 1); ++t) body(DA_BOOL(true), DA_BOOL(false), t);
+            for (; t + 1 < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+            body(DA_BOOL(false), DA_BOOL(true), t);
+        }
     }
-    if (row0 + l31 >= a.rows) return;
-    const float f2 = -da_lambda(a, head) * a.scale;
-    const size_t o = (((size_t)bi * a.nq + qi) * a.h + head) * W;
+    if (!ro.live) return;
+    const float f2 = -da_lambda(a, ro.head) * a.scale;
 #pragma unroll
     for (int j = 0; j < DB; ++j)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
             const int ch = 32 * j + 8 * g4 + 4 * lh;
-            f32x4 x, y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = g1[j][4 * g4 + i] * a.scale;
-                y[i] = g2[j][4 * g4 + i] * f2;
-            }
+            const f32x4 x = quad(g1[j], g4) * a.scale, y = quad(g2[j], g4) * f2;
             // D = 16: map 1 sits in channels 0..15 of its product, map 2 in channels 16..31 of its own
-            const int c1 = ch, c2 = D < 32 ? ch : D + ch;
             const bool ok1 = D >= 32 || ch < D, ok2 = D >= 32 || ch >= D;
             if (a.parts > 1) {
-                float* p = a.part + (size_t)part * a.b * a.nq * a.h * W + o;
-                if (ok1) *reinterpret_cast<f32x4*>(p + c1) = x;
-                if (ok2) *reinterpret_cast<f32x4*>(p + c2) = y;
+                float* p = a.part + (size_t)ro.part * a.b * a.nq * a.h * W + o;
+                if (ok1) *reinterpret_cast<f32x4*>(p + ch) = x;
+                if (ok2) *reinterpret_cast<f32x4*>(p + C2 + ch) = y;
             } else {
                 T* p = reinterpret_cast<T*>(a.dq) + o;
-                if (ok1) M::store4(p + c1, x);
-                if (ok2) M::store4(p + c2, y);
+                if (ok1) M::store4(p + ch, x);
+                if (ok2) M::store4(p + C2 + ch, y);
             }
         }
 }
 
-// dk, dv: a wave owns 32 keys and streams row tiles; row statistics come from LDS, four at a time.
+// dk, dv: a wave owns 32 keys and streams row tiles; the rows' constants come from LDS, four at a time.  Same pipeline as dq, with
+// q and dO read along rows in A (tile t + 1) and along columns in B (tile t): four buffers each.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     typedef Mx<T> M;
+    typedef typename M::Frag Frag;
     typedef Stager<T, D, 256> St;
-    constexpr int W = 2 * D, LD = St::LD, KC = D / 16, VC = W / 16, DB = (D + 31) / 32, CB = W / 32;
-    __shared__ __attribute__((aligned(16))) T Qs[2][DA_TILE * LD];
-    __shared__ __attribute__((aligned(16))) T Gs[2][DA_TILE * LD];
-    __shared__ __attribute__((aligned(16))) float Rs[2][6][DA_TILE];  // lse 1, lse 2, D_1, D_2, lambda, key limit (int)
+    constexpr int W = 2 * D, LD = St::LD, KC = D / 16, DB = (D + 31) / 32, CB = W / 32, C2 = D < 32 ? 0 : D;
+    __shared__ __attribute__((aligned(16))) T Qs[4][DA_TILE * LD];
+    __shared__ __attribute__((aligned(16))) T Gs[4][DA_TILE * LD];
+    __shared__ __attribute__((aligned(16))) float Rs[4][6][DA_TILE];  // lse 1, lse 2, D_1, D_2, lambda, key limit (int)
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lh = lane >> 5;
     const int tile = blockIdx.x % a.tiles;
@@ -681,7 +925,7 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     const bool live = key < a.nk && (!a.mask || a.mask[(size_t)bi * a.nk + min(key, a.nk - 1)]);
     const size_t n = (size_t)a.b * a.hk * a.rows;
 
-    typename M::Frag k1[KC], k2[KC], v[VC];
+    Frag k1[KC], k2[KC], v[2 * KC];
     {
         const int kc = min(key, a.nk - 1);
         const T* kp = reinterpret_cast<const T*>(a.k) + bi * a.k_sb + kh * a.k_sh + kc * a.k_sn;
@@ -690,144 +934,215 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
         for (int i = 0; i < KC; ++i) {
             k1[i] = live ? M::row(kp + 16 * i, lh) : M::zero();
             k2[i] = live ? M::row(kp + a.k_sm + 16 * i, lh) : M::zero();
+            v[2 * i] = live ? M::row(vp + 32 * i, lh) : M::zero();
+            v[2 * i + 1] = live ? M::row(vp + 32 * i + 16, lh) : M::zero();
         }
-#pragma unroll
-        for (int i = 0; i < VC; ++i) v[i] = live ? M::row(vp + 16 * i, lh) : M::zero();
     }
     int row_begin = part * a.span;
     const int row_end = min(a.rows, row_begin + a.span);
-    const int key_last = min(block0 + 128, a.nk);  // keys of the block: [block0, key_last)
-    if (a.frame) {  // the first query that sees the block's first key
-        const long long q0 = (long long)block0 / a.frame * a.frame - (a.nk - a.nq);
-        const long long r0 = q0 > 0 ? q0 * a.g / DA_TILE * DA_TILE : 0;
+    int nedge = 0;   // leading tiles with rows that do not see all of the workgroup's keys (rows see more and more of them)
+    if (a.frame) {
+        const long long shift = a.nk - a.nq, first = block0, last = min(block0 + 128, a.nk) - 1;
+        const long long q0 = first / a.frame * a.frame - shift, q1 = last / a.frame * a.frame - shift;
+        const long long r0 = q0 > 0 ? q0 * a.g / DA_TILE * DA_TILE : 0;  // the first row that sees the first key
         if (r0 > row_begin) row_begin = r0 < row_end ? (int)r0 : row_end;
+        const long long r1 = q1 * a.g - row_begin;  // the first row that sees the last key
+        nedge = r1 > 0 ? (int)min((r1 + DA_TILE - 1) / DA_TILE, (long long)INT_MAX) : 0;
     }
-    const T* qb = reinterpret_cast<const T*>(a.q) + bi * a.q_sb;
-    const T* gb = reinterpret_cast<const T*>(a.go) + (size_t)bi * a.nq * a.h * W;
+    const int ntiles = row_end > row_begin ? (row_end - row_begin + DA_TILE - 1) / DA_TILE : 0;
+    const char* qb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.q) + bi * a.q_sb + kh * a.g * a.q_sh);
+    const char* gb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.go) + ((size_t)bi * a.nq * a.h + kh * a.g) * W);
+    constexpr int E = (int)sizeof(T);
+    const unsigned q_sn = (unsigned)a.q_sn * E, q_sh = (unsigned)a.q_sh * E, g_sn = a.h * W * E, g_sh = W * E;
+    const unsigned gcol = St::col(tid) * E, qcol = (St::col(tid) >= D ? (unsigned)a.q_sm + St::col(tid) - D : St::col(tid)) * E;
 
-    St st;
+    St sq, sg;
     float rs = 0.f;
-    auto load_tile = [&](int r0) {
-        st.load(
-            tid,
-            [&](int r, int c, bool& ok) {
-                const int row = min(r0 + r, a.rows - 1);
-                ok = r0 + r < row_end;
-                return qb + row / a.g * a.q_sn + (kh * a.g + row % a.g) * a.q_sh + (c >= D ? a.q_sm + c - D : c);
-            },
-            [&](int r, int c) {
-                const int row = min(r0 + r, a.rows - 1);
-                return gb + ((size_t)(row / a.g) * a.h + kh * a.g + row % a.g) * W + c;
-            });
-        if (tid < 6 * DA_TILE) {
-            const int which = tid / DA_TILE, row = r0 + tid % DA_TILE;
-            const size_t e = (size_t)bh * a.rows + min(row, a.rows - 1);
-            if (which < 2)
-                rs = row < row_end ? a.lse[which * n + e] : DA_INF;  // rows past the end: weight 0
-            else if (which < 4)
-                rs = row < row_end ? a.delta[(which - 2) * n + e] : 0.f;
-            else if (which == 4)
-                rs = da_lambda(a, kh * a.g + min(row, a.rows - 1) % a.g);
-            else
-                rs = __int_as_float(da_limit(a, min(row, a.rows - 1)));
+    int stile = 0, srows = 0;  // first row of the tile in flight; how many rows the tile being put has
+    auto get = [&](int f, int t) {  // tiles past the end read the last row again
+        const int r0 = min(row_begin + t * DA_TILE, a.rows - 1), qi0 = da_div(a, r0);
+        const int row = min(r0 + St::row(tid, f), a.rows - 1), qi = da_div(a, row), g = row - qi * a.g;
+        sq.get(f, qb + qi0 * a.q_sn * E, (qi - qi0) * q_sn + g * q_sh + qcol);
+        sg.get(f, gb + (size_t)qi0 * a.h * W * E, (qi - qi0) * g_sn + g * g_sh + gcol);
+        if (f == 0) {
+            stile = row_begin + t * DA_TILE;
+            rs = a.stat[min(tid / DA_TILE, 5) * n + (size_t)bh * a.rows + min(stile + tid % DA_TILE, a.rows - 1)];
         }
     };
-    auto store_tile = [&](int buf) {
-        st.store(tid, Qs[buf], Gs[buf]);
-        if (tid < 6 * DA_TILE) Rs[buf][tid / DA_TILE][tid % DA_TILE] = rs;
+    auto put = [&](int f, int buf) {
+        if (f == 0) {
+            srows = row_end - stile;  // rows past the end: weight 0
+            Rs[buf][min(tid / DA_TILE, 5)][tid % DA_TILE] = (tid % DA_TILE >= srows) & (tid < 2 * DA_TILE) ? DA_INF : rs;
+        }
+        sq.put(tid, f, Qs[buf], St::row(tid, f) < srows);
+        sg.put(tid, f, Gs[buf], St::row(tid, f) < srows);
     };
-    f32x16 gk1[DB], gk2[DB], gv[CB];
+    f32x16 gk1[DB], gk2[DB], gv[CB], s1 = zero16(), s2 = zero16(), dp = zero16(), n1, n2, np;
 #pragma unroll
     for (int j = 0; j < DB; ++j) gk1[j] = gk2[j] = zero16();
 #pragma unroll
     for (int j = 0; j < CB; ++j) gv[j] = zero16();
+    Frag ga, gb_, gc, gd;  // the first operands of the next A
 
-    const int ntiles = row_end > row_begin ? (row_end - row_begin + DA_TILE - 1) / DA_TILE : 0;
-    if (ntiles > 0) {
-        load_tile(row_begin);
-        store_tile(0);
-        if (ntiles > 1) load_tile(row_begin + DA_TILE);
-    }
-    __syncthreads();
-    for (int t = 0; t < ntiles; ++t) {
-        const int cur = t & 1, r0 = row_begin + t * DA_TILE;
-        const T* Qc = Qs[cur] + l31 * LD;
-        const T* Gc = Gs[cur] + l31 * LD;
-        f32x16 s1 = zero16(), s2 = zero16(), dp = zero16();
+    auto ready = [&](int buf) {
+        n1 = n2 = np = zero16();
+        ga = M::row(Qs[buf] + l31 * LD, lh);
+        gb_ = M::row(Qs[buf] + l31 * LD + D, lh);
+        gc = M::row(Gs[buf] + l31 * LD, lh);
+        gd = M::row(Gs[buf] + l31 * LD + 16, lh);
+    };
+    auto body = [&](auto next, auto edge, int t) {
+        constexpr bool NEXT = decltype(next)::value;
+        const int b0 = t & 3, b1 = (t + 1) & 3, b2 = (t + 2) & 3;
+        const T *Qn = Qs[b1] + l31 * LD, *Gn = Gs[b1] + l31 * LD;
+        f32x16 mix;
+        f32x4 e1, e2, d1, d2, lam;
+        constexpr int SL = KC * M::STEPS;
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
-            M::mma(s1, M::row(Qc + 16 * i, lh), k1[i]);
-            M::mma(s2, M::row(Qc + D + 16 * i, lh), k2[i]);
-        }
+            const Frag fa = ga, fb = gb_, fc = gc, fd = gd;
+            if (NEXT && i + 1 < KC) {
+                ga = M::row(Qn + 16 * (i + 1), lh);
+                gb_ = M::row(Qn + D + 16 * (i + 1), lh);
+                gc = M::row(Gn + 32 * (i + 1), lh);
+                gd = M::row(Gn + 32 * (i + 1) + 16, lh);
+            }
 #pragma unroll
-        for (int i = 0; i < VC; ++i) M::mma(dp, M::row(Gc + 16 * i, lh), v[i]);
-        if (t + 1 < ntiles) {
-            store_tile(cur ^ 1);
-            if (t + 2 < ntiles) load_tile(r0 + 2 * DA_TILE);
-        }
-        const bool edge = a.frame && __float_as_int(Rs[cur][5][0]) < key_last;
-        f32x16 mix;
+            for (int e = 0; e < M::STEPS; ++e) {
+                if (NEXT) {
+                    M::step(n1, fa, k1[i], e);
+                    M::step(np, fc, v[2 * i], e);
+                    M::step(n2, fb, k2[i], e);
+                    M::step(np, fd, v[2 * i + 1], e);
+                }
+                const int slot = i * M::STEPS + e;
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-            const int o = 8 * g4 + 4 * lh;
-            const f32x4 e1 = *reinterpret_cast<const f32x4*>(&Rs[cur][0][o]), e2 = *reinterpret_cast<const f32x4*>(&Rs[cur][1][o]);
-            const f32x4 d1 = *reinterpret_cast<const f32x4*>(&Rs[cur][2][o]), d2 = *reinterpret_cast<const f32x4*>(&Rs[cur][3][o]);
-            const f32x4 lam = *reinterpret_cast<const f32x4*>(&Rs[cur][4][o]);
+                for (int r = slot * 16 / SL; r < (slot + 1) * 16 / SL; ++r) {
+                    const int o = 8 * (r >> 2) + 4 * lh, x = r & 3;
+                    if (x == 0) {
+                        e1 = *reinterpret_cast<const f32x4*>(&Rs[b0][0][o]);
+                        e2 = *reinterpret_cast<const f32x4*>(&Rs[b0][1][o]);
+                        d1 = *reinterpret_cast<const f32x4*>(&Rs[b0][2][o]);
+                        d2 = *reinterpret_cast<const f32x4*>(&Rs[b0][3][o]);
+                        lam = *reinterpret_cast<const f32x4*>(&Rs[b0][4][o]);
+                    }
+                    float p1 = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -e1[x])), p2 = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -e2[x]));
+                    if (decltype(edge)::value) {
+                        const bool hide = key >= __float_as_int(Rs[b0][5][o + x]);
+                        p1 = hide ? 0.f : p1;
+                        p2 = hide ? 0.f : p2;
+                    }
+                    p2 *= lam[x];
+                    mix[r] = p1 - p2;
+                    s1[r] = p1 * (dp[r] - d1[x]);
+                    s2[r] = p2 * (d2[x] - dp[r]);
+                }
+                if (NEXT) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 4 * g4 + i;
-                float p1 = __builtin_amdgcn_exp2f(fmaf(s1[r], a.c, -e1[i])), p2 = __builtin_amdgcn_exp2f(fmaf(s2[r], a.c, -e2[i]));
-                if (edge && key >= __float_as_int(Rs[cur][5][o + i])) p1 = p2 = 0.f;
-                p2 *= lam[i];
-                mix[r] = p1 - p2;
-                s1[r] = p1 * (dp[r] - d1[i]);
-                s2[r] = p2 * (d2[i] - dp[r]);
+                    for (int f = slot * St::F / SL; f < (slot + 1) * St::F / SL; ++f) {
+                        put(f, b2);
+                        get(f, t + 3);
+                    }
+                }
+                da_pin();
             }
         }
+        Frag nx = M::col(Gs[b0], LD, 0, 0, lane);
+        __syncthreads();
+        da_pin();
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
-            const typename M::Frag pm = M::reg(mix, t2), p1 = M::reg(s1, t2), p2 = M::reg(s2, t2);
+            const typename M::RegFrag pm = M::reg(mix, t2), p1 = M::reg(s1, t2), p2 = M::reg(s2, t2);
 #pragma unroll
-            for (int j = 0; j < CB; ++j) M::mma(gv[j], M::col(Gs[cur], LD, 16 * t2, 32 * j, lane), pm);
+            for (int j = 0; j < CB + 2 * DB; ++j) {  // dO's CB blocks, then the DB blocks of q_1 and of q_2
+                const Frag c = nx;
+                const int j1 = (j + 1) % (CB + 2 * DB), k0 = 16 * (t2 + (j + 1) / (CB + 2 * DB));
+                if (k0 < 32) {
+                    if (j1 < CB)
+                        nx = M::col(Gs[b0], LD, k0, 32 * j1, lane);
+                    else if (j1 < CB + DB)
+                        nx = M::col(Qs[b0], LD, k0, 32 * (j1 - CB), lane);
+                    else
+                        nx = M::col(Qs[b0], LD, k0, C2 + 32 * (j1 - CB - DB), lane);
+                }
 #pragma unroll
-            for (int j = 0; j < DB; ++j) {
-                M::mma(gk1[j], M::col(Qs[cur], LD, 16 * t2, 32 * j, lane), p1);
-                M::mma(gk2[j], M::col(Qs[cur], LD, 16 * t2, (D < 32 ? 0 : D) + 32 * j, lane), p2);
+                for (int e = 0; e < M::RSTEPS; ++e) {
+                    if (j < CB)
+                        M::rstep(gv[j < CB ? j : 0], c, pm, e);
+                    else if (j < CB + DB)
+                        M::rstep(gk1[j < CB + DB && j >= CB ? j - CB : 0], c, p1, e);
+                    else
+                        M::rstep(gk2[j >= CB + DB ? j - CB - DB : 0], c, p2, e);
+                }
+                da_pin();
             }
         }
+        if (NEXT) {
+            s1 = n1;
+            s2 = n2;
+            dp = np;
+            ready(b2);
+        }
+    };
+
+    if (ntiles > 0) {
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) get(f, 0);
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) put(f, 0);
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) get(f, 1);
         __syncthreads();
+        const T *Q0 = Qs[0] + l31 * LD, *G0 = Gs[0] + l31 * LD;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            const Frag fa = M::row(Q0 + 16 * i, lh), fb = M::row(Q0 + D + 16 * i, lh);
+            const Frag fc = M::row(G0 + 32 * i, lh), fd = M::row(G0 + 32 * i + 16, lh);
+#pragma unroll
+            for (int e = 0; e < M::STEPS; ++e) {
+                M::step(s1, fa, k1[i], e);
+                M::step(dp, fc, v[2 * i], e);
+                M::step(s2, fb, k2[i], e);
+                M::step(dp, fd, v[2 * i + 1], e);
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) {
+            put(f, 1);
+        }
+#pragma unroll
+        for (int f = 0; f < St::F; ++f) get(f, 2);
+        __syncthreads();
+        ready(1);
+        int t = 0;
+        if (M::ONE_LOOP) {
+            for (; t < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+        } else {
+            for (; t < min(nedge, ntiles - 1); ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+            for (; t + 1 < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(false), t);
+            body(DA_BOOL(false), DA_BOOL(true), t);
+        }
     }
     if (key >= a.nk) return;
     const size_t o = (((size_t)bi * a.nk + key) * a.hk + kh) * W;
-    const size_t np = (size_t)a.b * a.nk * a.hk * W;
-    auto put = [&](int which, int ch, f32x4 x) {
-        if (!live) x = f32x4{0.f, 0.f, 0.f, 0.f};  // its column never left this lane
+    const size_t all = (size_t)a.b * a.nk * a.hk * W;
+    auto out = [&](int which, int ch, f32x4 x) {
+        if (!live) x = f32x4{0.f, 0.f, 0.f, 0.f};  // whatever a hidden key's column holds, it never left this lane
         if (a.parts > 1)
-            *reinterpret_cast<f32x4*>(a.part + ((size_t)part * 2 + which) * np + o + ch) = x;
-        else if (which == 0)
-            M::store4(reinterpret_cast<T*>(a.dk) + o + ch, x);
+            *reinterpret_cast<f32x4*>(a.part + ((size_t)part * 2 + which) * all + o + ch) = x;
         else
-            M::store4(reinterpret_cast<T*>(a.dv) + o + ch, x);
+            M::store4(reinterpret_cast<T*>(which == 0 ? a.dk : a.dv) + o + ch, x);
     };
 #pragma unroll
     for (int g4 = 0; g4 < 4; ++g4) {
         const int c4 = 8 * g4 + 4 * lh;
-        f32x4 x;
 #pragma unroll
-        for (int j = 0; j < CB; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = gv[j][4 * g4 + i];
-            put(1, 32 * j + c4, x);
-        }
+        for (int j = 0; j < CB; ++j) out(1, 32 * j + c4, quad(gv[j], g4));
 #pragma unroll
         for (int j = 0; j < DB; ++j) {
             const int ch = 32 * j + c4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = gk1[j][4 * g4 + i] * a.scale;
-            if (D >= 32 || ch < D) put(0, ch, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = gk2[j][4 * g4 + i] * a.scale;
-            if (D >= 32 || ch >= D) put(0, D < 32 ? ch : D + ch, x);
+            if (D >= 32 || ch < D) out(0, ch, quad(gk1[j], g4) * a.scale);
+            if (D >= 32 || ch >= D) out(0, C2 + ch, quad(gk2[j], g4) * a.scale);
         }
     }
 }
@@ -910,11 +1225,11 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     // up to 32 rows: single-wave workgroups, many parts of the key axis; else four waves share a key tile
     p.wn = p.rows <= 32 ? 1 : 4;
     p.tiles = vspw_cdiv(p.rows, 32 * p.wn);
-    p.parts = p.wn == 1 ? da_parts(p.tiles * p.bhk, nt, 1024, 1, 256) : da_parts(p.tiles * p.bhk, nt, 512, 4, 32);
+    p.parts = p.wn == 1 ? da_parts(p.tiles * p.bhk, nt, 1024, 1, 256) : da_parts(p.tiles * p.bhk, nt, d->d == 64 ? 256 : 512, 4, 32);
     p.span = da_span(d->nk, p.parts);
     p.parts = vspw_cdiv(d->nk, p.span);
     p.fwd_bytes = p.parts > 1 ? (size_t)p.parts * p.bhk * p.rows * (2 * W + 4) * sizeof(float) : 0;
-    const int slots = d->dtype == VSPW_F32 ? 256 : 512;
+    const int slots = 256;
     p.qt = vspw_cdiv(p.rows, 128);
     p.qparts = da_parts(p.qt * p.bhk, nt, slots, 4, 16);
     p.qspan = da_span(d->nk, p.qparts);
@@ -935,15 +1250,21 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     size_t parts = 0;  // dq and dk/dv run one after the other and share the partial sums' memory
     if (p.qparts > 1) parts = (size_t)p.qparts * p.bhk * p.rows * W;
     if (p.kparts > 1 && (size_t)p.kparts * 2 * p.bhk * d->nk * W > parts) parts = (size_t)p.kparts * 2 * p.bhk * d->nk * W;
-    p.bwd_bytes = (size_t)bh * p.lchunks * sizeof(double) + ((size_t)2 * p.bhk * p.rows + parts) * sizeof(float);
+    p.bwd_bytes = (size_t)bh * p.lchunks * sizeof(double) + ((size_t)6 * p.bhk * p.rows + parts) * sizeof(float);
     p.bwd_bytes += 32;  // alignment of the pieces
     return true;
 }
-static bool da_strides_ok(const vspw_dattn_desc* d, const void* q, const void* k, const void* v) {
+#define DA_NEAR (1LL << 24)  // elements: 32 rows of a tile times 4 bytes stay below 2^31
+
+static bool da_strides_ok(const vspw_dattn_desc* d, const DaPlan& p, const void* q, const void* k, const void* v) {
     const long long ve = d->dtype == VSPW_F32 ? 4 : 8;
     const long long s[] = {d->q_sb, d->q_sn, d->q_sh, d->q_sm, d->k_sb, d->k_sn, d->k_sh, d->k_sm, d->v_sb, d->v_sn, d->v_sh};
     for (long long x : s)
         if (x % ve) return false;
+    const long long near[] = {d->q_sn, d->q_sh, d->q_sm, d->k_sn, d->k_sm, d->v_sn};  // offsets inside a tile are 32 bits
+    for (long long x : near)
+        if (x < 0 || x >= DA_NEAR) return false;
+    if (p.g > 1 && (long long)p.g * d->q_sh >= 4 * DA_NEAR) return false;
     return (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0;
 }
 static void da_fill(DaArgs& a, const vspw_dattn_desc* d, const DaPlan& p, const void* q, const void* k, const void* v,
@@ -977,6 +1298,10 @@ static void da_fill(DaArgs& a, const vspw_dattn_desc* d, const DaPlan& p, const 
     a.lchunks = p.lchunks;
     a.scale = d->scale;
     a.c = d->scale * 1.4426950408889634f;
+    unsigned l = 0;  // 2^l >= g: gm = ceil(2^(31 + l) / g) is off by less than 2^l / g, exact for 31-bit x
+    while ((1ull << l) < (unsigned)p.g) ++l;
+    a.gs = 31 + l;
+    a.gm = (unsigned)(((1ull << a.gs) + p.g - 1) / p.g);
 }
 
 extern "C" size_t vspw_diff_attn_fwd_workspace(const vspw_dattn_desc* d) {
@@ -988,6 +1313,8 @@ extern "C" size_t vspw_diff_attn_bwd_workspace(const vspw_dattn_desc* d) {
     return da_plan(d, p) ? p.bwd_bytes : 0;
 }
 
+#define DA_JOIN_PARTS 32
+
 template <typename T, int D>
 static int da_fwd_launch(const DaArgs& a, const DaPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)(p.tiles * p.bhk * p.parts));
@@ -997,7 +1324,11 @@ static int da_fwd_launch(const DaArgs& a, const DaPlan& p, hipStream_t st) {
         hipLaunchKernelGGL((da_fwd_kernel<T, D, 4>), grid, dim3(256), 0, st, a);
     const int rc = vspw_launch_status();
     if (rc != VSPW_OK || p.parts == 1) return rc;
-    hipLaunchKernelGGL((da_join_kernel<T, D>), dim3((unsigned)(p.bhk * p.rows)), dim3(256), 0, st, a);
+    const long long rows = p.bhk * p.rows;
+    if (p.parts > DA_JOIN_PARTS)
+        hipLaunchKernelGGL((da_join_row_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((da_join_kernel<T, D>), dim3((unsigned)vspw_cdiv(rows, 256 / (D / 2))), dim3(256), 0, st, a);
     return vspw_launch_status();
 }
 
@@ -1049,15 +1380,15 @@ static int da_bwd_launch(DaArgs a, const DaPlan& p, hipStream_t st) {
                                         : d->d == 32 ? FN<bf16_t, 32>(__VA_ARGS__) : FN<bf16_t, 64>(__VA_ARGS__)))
 
 extern "C" int vspw_diff_attn_fwd(const vspw_dattn_desc* d, const void* q, const void* k, const void* v, const void* lam,
-                                  const unsigned char* key_mask, void* out, void* o2, float* lse, void* ws, size_t ws_bytes,
+                                  const unsigned char* key_mask, void* out, float* maps, float* lse, void* ws, size_t ws_bytes,
                                   void* stream) {
     DaPlan p;
-    if (!q || !k || !v || !lam || !out || !da_plan(d, p) || !da_strides_ok(d, q, k, v)) return VSPW_EINVAL;
-    if ((((uintptr_t)out | (uintptr_t)o2 | (uintptr_t)ws) & 15) || ws_bytes < p.fwd_bytes || (p.fwd_bytes && !ws)) return VSPW_EINVAL;
+    if (!q || !k || !v || !lam || !out || !da_plan(d, p) || !da_strides_ok(d, p, q, k, v)) return VSPW_EINVAL;
+    if ((((uintptr_t)out | (uintptr_t)maps | (uintptr_t)ws) & 15) || ws_bytes < p.fwd_bytes || (p.fwd_bytes && !ws)) return VSPW_EINVAL;
     DaArgs a;
     da_fill(a, d, p, q, k, v, lam, key_mask);
     a.out = out;
-    a.o2 = o2;
+    a.maps = maps;
     a.lse = lse;
     a.tiles = p.tiles;
     a.parts = p.parts;
@@ -1068,29 +1399,28 @@ extern "C" int vspw_diff_attn_fwd(const vspw_dattn_desc* d, const void* q, const
 }
 
 extern "C" int vspw_diff_attn_bwd(const vspw_dattn_desc* d, const void* q, const void* k, const void* v, const void* lam,
-                                  const unsigned char* key_mask, const void* out, const void* o2, const float* lse,
-                                  const void* go, void* dq, void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes,
+                                  const unsigned char* key_mask, const float* maps, const float* lse, const void* go,
+                                  void* dq, void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes,
                                   void* stream) {
     DaPlan p;
-    if (!q || !k || !v || !lam || !out || !o2 || !lse || !go || !da_plan(d, p) || !da_strides_ok(d, q, k, v)) return VSPW_EINVAL;
+    if (!q || !k || !v || !lam || !maps || !lse || !go || !da_plan(d, p) || !da_strides_ok(d, p, q, k, v)) return VSPW_EINVAL;
     if ((dk == nullptr) != (dv == nullptr) || !ws || ws_bytes < p.bwd_bytes) return VSPW_EINVAL;
-    if (((uintptr_t)out | (uintptr_t)o2 | (uintptr_t)go | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)
+    if (((uintptr_t)maps | (uintptr_t)go | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)
         return VSPW_EINVAL;
     DaArgs a;
     da_fill(a, d, p, q, k, v, lam, key_mask);
-    a.out = const_cast<void*>(out);
-    a.o2 = const_cast<void*>(o2);
+    a.maps = const_cast<float*>(maps);
     a.lse = const_cast<float*>(lse);
     a.go = go;
     a.dq = dq;
     a.dk = dk;
     a.dv = dv;
     a.dlam = dlam;
-    // [lpart doubles][delta][partial sums], every piece on 16 bytes
+    // [lpart doubles][stat][partial sums], every piece on 16 bytes
     a.lpart = reinterpret_cast<double*>(ws);
     size_t off = ((size_t)d->b * d->h * p.lchunks * sizeof(double) + 15) / 16 * 16;
-    a.delta = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + off);
-    off += ((size_t)2 * p.bhk * p.rows * sizeof(float) + 15) / 16 * 16;
+    a.stat = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + off);
+    off += ((size_t)6 * p.bhk * p.rows * sizeof(float) + 15) / 16 * 16;
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + off);
     return DA_DISPATCH(da_bwd_launch, a, p, vspw_stream(stream));
 }

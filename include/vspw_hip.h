@@ -653,8 +653,8 @@ int vspw_group_norm_bwd(const void* x, const void* dy, void* dx, int n, long lon
  *   lam [h] of lam_dtype (fp32 or bf16);  key_mask [b][nk] bytes (0: the key takes no part), may be NULL
  *   frame > 0: query i sees keys j with j / frame <= (i + nk - nq) / frame (its frame and earlier ones); 0: all keys
  *   scale > 0.  A row without visible keys is zero, with zero gradients; what masked keys and values hold is not used.
- * out, o2, go [b][nq][h][2d], dq [b][nq][h][2][d], dk / dv like contiguous k / v.  For the backward pass the forward call
- * writes o2 (the second map's output) and lse (fp32 [2][b * hk * nq * h / hk]); both NULL at inference.
+ * out, go [b][nq][h][2d], dq [b][nq][h][2][d], dk / dv like contiguous k / v.  For the backward pass the forward call
+ * writes maps (fp32 [b][nq][h][2][2d], both maps' outputs) and lse (fp32 [2][b * hk * nq * h / hk]); both NULL at inference.
  * dq, (dk and dv), dlam may each be NULL.  Results do not depend on the run: every sum has a fixed order. */
 typedef struct vspw_dattn_desc {
     int b, nq, nk, h, hk, d, dtype, lam_dtype, frame;
@@ -663,12 +663,12 @@ typedef struct vspw_dattn_desc {
 } vspw_dattn_desc;
 size_t vspw_diff_attn_fwd_workspace(const vspw_dattn_desc* d);
 int vspw_diff_attn_fwd(const vspw_dattn_desc* d, const void* q, const void* k, const void* v, const void* lam,
-                       const unsigned char* key_mask, void* out, void* o2, float* lse, void* ws, size_t ws_bytes,
+                       const unsigned char* key_mask, void* out, float* maps, float* lse, void* ws, size_t ws_bytes,
                        void* stream);
 size_t vspw_diff_attn_bwd_workspace(const vspw_dattn_desc* d);
 int vspw_diff_attn_bwd(const vspw_dattn_desc* d, const void* q, const void* k, const void* v, const void* lam,
-                       const unsigned char* key_mask, const void* out, const void* o2, const float* lse, const void* go,
-                       void* dq, void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
+                       const unsigned char* key_mask, const float* maps, const float* lse, const void* go, void* dq,
+                       void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
 /* lam[i] = exp(lq1[i].lk1[i]) - exp(lq2[i].lk2[i]) + init for fp32 [h][d] vectors: the learned weight of the second map;
  * _bwd: the gradients of the four vectors from g [h]. */
 int vspw_diff_lambda_fwd(const float* lq1, const float* lk1, const float* lq2, const float* lk2, float init, float* lam, int h,

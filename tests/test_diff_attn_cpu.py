@@ -68,10 +68,10 @@ def test_c_entry_points_refuse_bad_arguments():
     assert _C.query("vspw_diff_attn_fwd_workspace", ctypes.byref(big)) > 0
     assert fwd(big, ws=None) == -1 and fwd(big, n=8) == -1 and fwd(big, ws=odd) == -1
 
-    def bwd(d=None, lse=p, o2=p, dk=p, dv=p, ws=p, n=1 << 30):
-        return lib.vspw_diff_attn_bwd(ctypes.byref(d or desc()), p, p, p, p, None, p, o2, lse, p, p, dk, dv, p, ws, n, None)
+    def bwd(d=None, lse=p, maps=p, dk=p, dv=p, ws=p, n=1 << 30):
+        return lib.vspw_diff_attn_bwd(ctypes.byref(d or desc()), p, p, p, p, None, maps, lse, p, p, dk, dv, p, ws, n, None)
 
-    for kw in (dict(lse=None), dict(o2=None), dict(dk=None), dict(dv=None), dict(ws=None), dict(n=8), dict(d=desc(d=20))):
+    for kw in (dict(lse=None), dict(maps=None), dict(dk=None), dict(dv=None), dict(ws=None), dict(n=8), dict(d=desc(d=20))):
         assert bwd(**kw) == -1, kw
     assert lib.vspw_diff_lambda_fwd(p, p, p, p, 0.1, None, 1, 4, None) == -1
     assert lib.vspw_diff_lambda_fwd(p, p, p, p, 0.1, p, 0, 4, None) == -1
