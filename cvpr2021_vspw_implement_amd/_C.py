@@ -119,17 +119,27 @@ def check(rc: int, what: str):
 trace = None  # optional callable(name, args) -> context manager (ops.kernel_timer: HIP events around HBM-bound kernels)
 
 
+_fns = {}  # entry points by name (a ctypes attribute lookup costs as much as a small call)
+
+
+def _fn(name: str):
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
+    return fn
+
+
 def call(name: str, *args):
     """Call an int-returning entry point and raise on a non-zero status."""
     if trace is not None:
         with trace(name, args):
-            rc = getattr(load(), name)(*args)
+            rc = _fn(name)(*args)
     else:
-        rc = getattr(load(), name)(*args)
+        rc = _fn(name)(*args)
     if rc != 0:
         check(rc, name)
 
 
 def query(name: str, *args):
     """Call a size_t-returning *_workspace()/partials() entry point."""
-    return getattr(load(), name)(*args)
+    return _fn(name)(*args)

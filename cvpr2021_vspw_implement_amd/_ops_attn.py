@@ -6,8 +6,8 @@ import math
 import torch
 
 from . import _C
-from ._ops_norm import _DTYPES, _on, _require_float, _same_device
-from ._opbase import _p, _stream, _Timed, _ws
+from ._ops_norm import _DTYPES, _addr, _on_device, _raw_stream, _require_float, _same_device, _wants_grad
+from ._opbase import _Timed, _ktimer, _ws
 
 _ATTN_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -21,30 +21,96 @@ class AttnDesc(ctypes.Structure):
                                                     "v_sb", "v_sn", "v_sh")])
 
 
-def _strided(t):
-    """t itself when the kernels can address it (dense last dimension, everything else on 16 bytes), else a copy."""
-    ve = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-    ok = ok and all(n == 1 or s % ve == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+_NEAR = 1 << 24  # strides between rows, maps and heads that the kernels address with 32 bits inside a tile (elements)
 
 
 def _strides(t):
+    """Element strides of all dimensions but the last, 0 where there is nothing to step over."""
     return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
 
 
-def _desc(q, k, v, lam, scale, frame):
+def _strided(t, g=1):
+    """(t, its strides) when the kernels can address it (dense last dimension, everything else on 16 bytes, near rows), else of
+    a copy.  g: how many heads a tile of rows mixes."""
+    st = _strides(t)
+    ve = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    for i, s in enumerate(st):
+        ok = ok and s % ve == 0 and (i == 0 or (i == 2 and g == 1) or s * (g if i == 2 else 1) < _NEAR)
+    if not ok:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _strides(t)
+    return t, st
+
+
+def _desc(q, k, lam, scale, frame, qs, ks, vs):
     b, nq, h, _, d = q.shape
-    qs, ks, vs = _strides(q), _strides(k), _strides(v)
     return AttnDesc(b, nq, k.shape[1], h, k.shape[2], d, _ATTN_DTYPES[q.dtype], _ATTN_DTYPES[lam.dtype], frame, scale,
                     *qs, *ks, *vs)
 
 
-def _pairs(q, k, frame):
-    nq, nk = q.shape[1], k.shape[1]
-    if not frame:
-        return float(nq) * nk
-    return float(nk) * nq - 0.5 * nq * max(0, min(nq, nk) - frame)  # for the launch timers: the mean of the visible keys
+def _flops(q, k, frame, per_pair):
+    """For the launch timers: the mean of the visible keys."""
+    b, nq, h, _, d = q.shape
+    nk = k.shape[1]
+    pairs = float(nk) * nq - (0.5 * nq * max(0, min(nq, nk) - frame) if frame else 0.0)
+    return per_pair * b * h * d * pairs
+
+
+def _timed(name, q, k, frame, per_pair):
+    if not _ktimer["on"]:
+        return _Timed(name, 0.0)
+    return _Timed(name, _flops(q, k, frame, per_pair), "diff_attn b%d n%d/%d h%d d%d" % (q.shape[0], q.shape[1], k.shape[1],
+                                                                                          q.shape[2], q.shape[4]))
+
+
+@_on_device
+def _attn_fwd(q, k, v, lam, scale, mask, frame, train):
+    """(out, maps, lse, descriptor, q, k, v): the last three as the kernels read them"""
+    hk = k.shape[2]
+    b, nq, h, _, d = q.shape
+    (q, qs), (k, ks), (v, vs) = _strided(q, h // hk), _strided(k), _strided(v)
+    out = torch.empty((b, nq, h, 2 * d), device=q.device, dtype=q.dtype)
+    maps = lse = None
+    if not out.numel() or not k.shape[1]:
+        return out.zero_(), None, None, None, q, k, v
+    if train:
+        maps = torch.empty((b, nq, h, 2, 2 * d), device=q.device, dtype=torch.float32)
+        lse = torch.empty((2, b * hk, nq * (h // hk)), device=q.device, dtype=torch.float32)
+    ds = _desc(q, k, lam, scale, frame, qs, ks, vs)
+    ref = ctypes.byref(ds)
+    nbytes = _C.query("vspw_diff_attn_fwd_workspace", ref)
+    ws = _ws(nbytes, q.device) if nbytes else None
+    with _timed("diff_attn_fwd", q, k, frame, 12.0):
+        _C.call("vspw_diff_attn_fwd", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(mask), out.data_ptr(),
+                _addr(maps), _addr(lse), _addr(ws), nbytes, _raw_stream(q.device.index))
+    return out, maps, lse, ds, q, k, v
+
+
+@_on_device
+def _attn_bwd(q, k, v, lam, mask, maps, lse, ds, go, frame, need):
+    dev, dt = q.device, q.dtype
+    dq = torch.empty(q.shape, device=dev, dtype=dt) if need[0] else None
+    dk = dv = None
+    if need[1] or need[2]:
+        dk, dv = torch.empty(k.shape, device=dev, dtype=dt), torch.empty(v.shape, device=dev, dtype=dt)
+    dlam = torch.empty_like(lam) if need[3] else None
+    if maps is None:  # no rows or no keys
+        for t in (dq, dk, dv, dlam):
+            if t is not None:
+                t.zero_()
+        return dq, dk, dv, dlam
+    go = go.contiguous()
+    if go.data_ptr() % 16:
+        go = go.clone()
+    ref = ctypes.byref(ds)
+    nbytes = _C.query("vspw_diff_attn_bwd_workspace", ref)
+    ws = _ws(nbytes, dev)
+    with _timed("diff_attn_bwd", q, k, frame, 28.0):
+        _C.call("vspw_diff_attn_bwd", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(mask), maps.data_ptr(),
+                lse.data_ptr(), go.data_ptr(), _addr(dq), _addr(dk), _addr(dv), _addr(dlam), ws.data_ptr(), nbytes,
+                _raw_stream(dev.index))
+    return dq, dk, dv, dlam
 
 
 class DiffAttentionFn(torch.autograd.Function):
@@ -52,53 +118,17 @@ class DiffAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lam, scale, mask, frame):
-        q, k, v = _strided(q), _strided(k), _strided(v)
-        b, nq, h, _, d = q.shape
-        nk, hk = k.shape[1], k.shape[2]
-        train = any(ctx.needs_input_grad[:4])
-        out = torch.empty((b, nq, h, 2 * d), device=q.device, dtype=q.dtype)
-        maps = lse = None
-        if out.numel() and nk:
-            with _on(q):
-                if train:
-                    maps = torch.empty((b, nq, h, 2, 2 * d), device=q.device, dtype=torch.float32)
-                    lse = torch.empty((2, b * hk, nq * (h // hk)), device=q.device, dtype=torch.float32)
-                ds = _desc(q, k, v, lam, scale, frame)
-                nbytes = _C.query("vspw_diff_attn_fwd_workspace", ctypes.byref(ds))
-                ws = _ws(nbytes, q.device) if nbytes else None
-                with _Timed("diff_attn_fwd", 12.0 * b * h * d * _pairs(q, k, frame), "diff_attn b%d n%d/%d h%d d%d" % (b, nq, nk, h, d)):
-                    _C.call("vspw_diff_attn_fwd", ctypes.byref(ds), _p(q), _p(k), _p(v), _p(lam), _p(mask), _p(out), _p(maps),
-                            _p(lse), _p(ws), nbytes, _stream())
-        else:
-            out.zero_()
-        ctx.meta = (scale, frame)
+        out, maps, lse, ds, q, k, v = _attn_fwd(q, k, v, lam, scale, mask, frame, True)
+        ctx.meta = (ds, frame)
         ctx.save_for_backward(q, k, v, lam, mask, maps, lse)
         return out
 
     @staticmethod
     def backward(ctx, go):
         q, k, v, lam, mask, maps, lse = ctx.saved_tensors
-        scale, frame = ctx.meta
+        ds, frame = ctx.meta
         need = ctx.needs_input_grad
-        b, nq, h, _, d = q.shape
-        nk = k.shape[1]
-        with _on(q):
-            dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need[0] else None
-            dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if need[1] or need[2] else None
-            dv = torch.empty(v.shape, device=q.device, dtype=q.dtype) if need[1] or need[2] else None
-            dlam = torch.empty_like(lam) if need[3] else None
-            if maps is None:  # no rows or no keys
-                for t in (dq, dk, dv, dlam):
-                    if t is not None:
-                        t.zero_()
-            else:
-                go = _strided(go.contiguous())
-                ds = _desc(q, k, v, lam, scale, frame)
-                nbytes = _C.query("vspw_diff_attn_bwd_workspace", ctypes.byref(ds))
-                ws = _ws(nbytes, q.device)
-                with _Timed("diff_attn_bwd", 28.0 * b * h * d * _pairs(q, k, frame), "diff_attn b%d n%d/%d h%d d%d" % (b, nq, nk, h, d)):
-                    _C.call("vspw_diff_attn_bwd", ctypes.byref(ds), _p(q), _p(k), _p(v), _p(lam), _p(mask), _p(maps),
-                            _p(lse), _p(go), _p(dq), _p(dk), _p(dv), _p(dlam), _p(ws), nbytes, _stream())
+        dq, dk, dv, dlam = _attn_bwd(q, k, v, lam, mask, maps, lse, ds, go, frame, need)
         return dq, dk if need[1] else None, dv if need[2] else None, dlam, None, None, None
 
 
@@ -149,28 +179,40 @@ def diff_attention(q, k, v, lam, scale=None, key_mask=None, frame=0):
             raise RuntimeError("diff_attention: key_mask must be bool [%d,%d], got %s %s"
                                % (b, nk, key_mask.dtype, tuple(key_mask.shape)))
         key_mask = key_mask.contiguous()
-    return DiffAttentionFn.apply(q, k, v, lam.contiguous(), scale, key_mask, frame)
+    lam = lam.contiguous()
+    if _wants_grad(q, k, v, lam):
+        return DiffAttentionFn.apply(q, k, v, lam, scale, key_mask, frame)
+    return _attn_fwd(q, k, v, lam, scale, key_mask, frame, False)[0]
+
+
+@_on_device
+def _lambda_fwd(lq1, lk1, lq2, lk2, init):
+    h, d = lq1.shape
+    lam = torch.empty(h, device=lq1.device, dtype=torch.float32)
+    _C.call("vspw_diff_lambda_fwd", lq1.data_ptr(), lk1.data_ptr(), lq2.data_ptr(), lk2.data_ptr(), init, lam.data_ptr(), h, d,
+            _raw_stream(lq1.device.index))
+    return lam
+
+
+@_on_device
+def _lambda_bwd(lq1, lk1, lq2, lk2, g):
+    h, d = lq1.shape
+    g = g.contiguous()
+    grads = [torch.empty_like(lq1) for _ in range(4)]
+    _C.call("vspw_diff_lambda_bwd", lq1.data_ptr(), lk1.data_ptr(), lq2.data_ptr(), lk2.data_ptr(), g.data_ptr(),
+            *[t.data_ptr() for t in grads], h, d, _raw_stream(lq1.device.index))
+    return tuple(grads)
 
 
 class DiffLambdaFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, lq1, lk1, lq2, lk2, init):
-        h, d = lq1.shape
-        lam = torch.empty(h, device=lq1.device, dtype=torch.float32)
-        with _on(lq1):
-            _C.call("vspw_diff_lambda_fwd", _p(lq1), _p(lk1), _p(lq2), _p(lk2), init, _p(lam), h, d, _stream())
         ctx.save_for_backward(lq1, lk1, lq2, lk2)
-        return lam
+        return _lambda_fwd(lq1, lk1, lq2, lk2, init)
 
     @staticmethod
     def backward(ctx, g):
-        lq1, lk1, lq2, lk2 = ctx.saved_tensors
-        h, d = lq1.shape
-        grads = [torch.empty_like(lq1) for _ in range(4)]
-        with _on(lq1):
-            _C.call("vspw_diff_lambda_bwd", _p(lq1), _p(lk1), _p(lq2), _p(lk2), _p(g.float().contiguous()),
-                    *[_p(t) for t in grads], h, d, _stream())
-        return tuple(grads) + (None,)
+        return _lambda_bwd(*ctx.saved_tensors, g) + (None,)
 
 
 def diff_lambda(lq1, lk1, lq2, lk2, init):

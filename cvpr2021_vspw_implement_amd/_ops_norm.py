@@ -4,15 +4,24 @@ the operators of ops.py that take float32, bfloat16 and float16 activations.
 Both work on channels-last memory like the rest of ops.py: a [N,C,...] tensor is brought to [N][pixels][C] order (zero-copy
 when it is already there) and the result comes back in that order under the input's logical shape.
 """
-import contextlib
+import functools
 
 import torch
 
 from . import _C
-from ._opbase import _p, _stream, _ws, is_nhwc, to_nhwc
+from ._opbase import _ws, to_nhwc
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # VSPW_F32 / VSPW_BF16 / VSPW_F16
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+# These operators are called on small tensors too, where the host decides: addresses and streams go to ctypes as integers,
+# and calls that need no gradient do not pass through autograd.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _require_float(t, what, dtypes=_DTYPES):
@@ -24,23 +33,38 @@ def _require_float(t, what, dtypes=_DTYPES):
 
 
 def _same_device(what, first, *others):
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError("%s: tensors on %s and %s" % (what, first.device, t.device))
+        if t is not None and t.device != dev:
+            raise RuntimeError("%s: tensors on %s and %s" % (what, dev, t.device))
 
 
-def _on(t):
-    """The tensor's device as the current one: kernels run on ITS device's current stream."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _on_device(fn):
+    """fn(t, ...) with t's device as the current one: kernels run on ITS device's current stream."""
+
+    @functools.wraps(fn)
+    def run(t, *args):
+        if t.device.index == _current_device():
+            return fn(t, *args)
+        with torch.cuda.device(t.device):
+            return fn(t, *args)
+
+    return run
+
+
+def _wants_grad(*ts):
+    if not torch.is_grad_enabled():
+        return False
+    for t in ts:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _rows(x):
     """[N,C,...] of any strides -> ([N][pixels][C] memory under the logical shape [N,C,P,1], its 4-D tensor)."""
-    n, c = x.shape[0], x.shape[1]
-    x4 = x if x.dim() == 4 else x.reshape(n, c, -1, 1)
-    if is_nhwc(x4):
+    x4 = x if x.dim() == 4 else x.reshape(x.shape[0], x.shape[1], -1, 1)
+    if x4.is_contiguous(memory_format=torch.channels_last):
         return x4
     if x4.dtype == torch.float32 and x4.is_contiguous() and x4.numel():
         return to_nhwc(x4)
@@ -63,38 +87,35 @@ def _check_rng(what, p, rng):
     return p
 
 
-def _drop(x, p, rng, channelwise, dims):
-    y = torch.empty_like(x)  # preserves the dense memory order
-    n, hw, c = dims
-    if x.numel():
-        _C.call("vspw_dropout", _p(x), _p(y), n, hw, c, _DTYPES[x.dtype], p, _p(rng), 1 if channelwise else 0, _stream())
-    return y
+# ------------------------------------------------------------------------------------------------------------ dropout
+@_on_device
+def _dropout(x, p, rng, channelwise):
+    shape = x.shape
+    nd = len(shape)
+    if nd >= 3:
+        xr = _rows(x)
+        n, c, h, w = xr.shape
+        hw = h * w
+    else:
+        xr = x.contiguous()
+        n, hw, c = (shape[0], 1, shape[1]) if channelwise else (1, xr.numel(), 1)
+    y = torch.empty_like(xr)  # preserves the dense memory order
+    if xr.numel():
+        _C.call("vspw_dropout", xr.data_ptr(), y.data_ptr(), n, hw, c, _DTYPES[x.dtype], p, rng.data_ptr(),
+                1 if channelwise else 0, _raw_stream(x.device.index))
+    return y if nd == 4 else y.reshape(shape)
 
 
 class DropoutFn(torch.autograd.Function):
     @staticmethod
-    def _launch(x, p, rng, channelwise):
-        if x.dim() >= 3:
-            xr = _rows(x)
-            dims = (xr.shape[0], xr.shape[2] * xr.shape[3], xr.shape[1])
-        else:
-            xr = x.contiguous()
-            dims = (x.shape[0], 1, x.shape[1]) if channelwise else (1, xr.numel(), 1)
-        return _drop(xr, p, rng, channelwise, dims).reshape(x.shape)
-
-    @staticmethod
     def forward(ctx, x, p, rng, channelwise):
-        with _on(x):
-            y = DropoutFn._launch(x, p, rng, channelwise)
         ctx.meta = (p, channelwise)
         ctx.save_for_backward(rng)
-        return y
+        return _dropout(x, p, rng, channelwise)
 
     @staticmethod
     def backward(ctx, g):
-        (rng,) = ctx.saved_tensors
-        with _on(g):
-            return DropoutFn._launch(g, ctx.meta[0], rng, ctx.meta[1]), None, None, None
+        return _dropout(g, ctx.meta[0], ctx.saved_tensors[0], ctx.meta[1]), None, None, None
 
 
 def dropout(x, p, rng=None, channelwise=False):
@@ -111,7 +132,16 @@ def dropout(x, p, rng=None, channelwise=False):
     _same_device("dropout", x, rng)
     if channelwise and x.dim() < 2:
         raise RuntimeError("dropout: channelwise needs a [N,C,...] tensor, got %s" % (tuple(x.shape),))
-    return DropoutFn.apply(x, p, rng, bool(channelwise))
+    if _wants_grad(x):
+        return DropoutFn.apply(x, p, rng, bool(channelwise))
+    return _dropout(x, p, rng, channelwise)
+
+
+@_on_device
+def _rng_next(state):
+    used = torch.empty_like(state)
+    _C.call("vspw_rng_next", state.data_ptr(), used.data_ptr(), _raw_stream(state.device.index))
+    return used
 
 
 def rng_next(state):
@@ -119,10 +149,55 @@ def rng_next(state):
     advances by one - on the stream, so every replay of a captured step draws a new mask."""
     if not state.is_cuda or state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous():
         raise RuntimeError("rng_next: two contiguous int64 values (seed, offset) on the GPU expected")
-    used = torch.empty_like(state)
-    with _on(state):
-        _C.call("vspw_rng_next", _p(state), _p(used), _stream())
-    return used
+    return _rng_next(state)
+
+
+# --------------------------------------------------------------------------------------------------------- group norm
+@functools.lru_cache(maxsize=None)
+def _norm_workspace(which, n, hw, c, groups, dt):
+    return _C.query("vspw_group_norm_%s_workspace" % which, n, hw, c, groups, dt)
+
+
+@_on_device
+def _norm_fwd(x, weight, bias, groups, eps, act, p, rng, channelwise, train):
+    """(y, rows of x, stats)"""
+    xr = _aligned(_rows(x))
+    n, c, h, w = xr.shape
+    hw = h * w
+    dt = _DTYPES[x.dtype]
+    y = torch.empty_like(xr)
+    stats = torch.empty((n, groups, 2), device=x.device, dtype=torch.float64) if train else None
+    if xr.numel():
+        nbytes = _norm_workspace("fwd", n, hw, c, groups, dt)
+        ws = _ws(nbytes, x.device) if nbytes else None
+        _C.call("vspw_group_norm_fwd", xr.data_ptr(), y.data_ptr(), n, hw, c, groups, dt, _addr(weight), _addr(bias), eps, act, p,
+                _addr(rng), channelwise, _addr(stats), _addr(ws), nbytes, _raw_stream(x.device.index))
+    return (y if x.dim() == 4 else y.reshape(x.shape)), xr, stats
+
+
+@_on_device
+def _norm_bwd(xr, g, weight, bias, rng, stats, meta, need):
+    groups, act, p, channelwise, shape = meta
+    n, c, h, w = xr.shape
+    hw = h * w
+    dt = _DTYPES[xr.dtype]
+    gr = _aligned(_rows(g))
+    dx = torch.empty_like(xr) if need[0] else None
+    dw = torch.empty_like(weight) if need[1] else None
+    db = torch.empty_like(bias) if need[2] else None
+    if xr.numel():
+        nbytes = _norm_workspace("bwd", n, hw, c, groups, dt)
+        ws = _ws(nbytes, xr.device)
+        _C.call("vspw_group_norm_bwd", xr.data_ptr(), gr.data_ptr(), _addr(dx), n, hw, c, groups, dt, _addr(weight), _addr(bias),
+                act, p, _addr(rng), channelwise, stats.data_ptr(), _addr(dw), _addr(db), ws.data_ptr(), nbytes,
+                _raw_stream(xr.device.index))
+    else:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    if dx is not None and len(shape) != 4:
+        dx = dx.reshape(shape)
+    return dx, dw, db
 
 
 class GroupNormActFn(torch.autograd.Function):
@@ -130,46 +205,15 @@ class GroupNormActFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act, p, rng, channelwise):
-        xr = _aligned(_rows(x))
-        n, c, h, w = xr.shape
-        hw = h * w
-        dt = _DTYPES[x.dtype]
-        y = torch.empty_like(xr)
-        train = any(ctx.needs_input_grad[:3])
-        with _on(x):
-            stats = torch.empty((n, groups, 2), device=x.device, dtype=torch.float64) if train else None
-            if xr.numel():
-                nbytes = _C.query("vspw_group_norm_fwd_workspace", n, hw, c, groups, dt)
-                ws = _ws(nbytes, x.device)
-                _C.call("vspw_group_norm_fwd", _p(xr), _p(y), n, hw, c, groups, dt, _p(weight), _p(bias), eps, act, p,
-                        _p(rng), channelwise, _p(stats), _p(ws), nbytes, _stream())
-        ctx.meta = (groups, act, p, channelwise, tuple(x.shape))
+        y, xr, stats = _norm_fwd(x, weight, bias, groups, eps, act, p, rng, channelwise, True)
+        ctx.meta = (groups, act, p, channelwise, x.shape)
         ctx.save_for_backward(xr, weight, bias, rng, stats)
-        return y.reshape(x.shape)
+        return y
 
     @staticmethod
     def backward(ctx, g):
         xr, weight, bias, rng, stats = ctx.saved_tensors
-        groups, act, p, channelwise, shape = ctx.meta
-        n, c, h, w = xr.shape
-        hw = h * w
-        dt = _DTYPES[xr.dtype]
-        need = ctx.needs_input_grad
-        with _on(xr):
-            gr = _aligned(_rows(g))
-            dx = torch.empty_like(xr) if need[0] else None
-            dw = torch.empty_like(weight) if need[1] else None
-            db = torch.empty_like(bias) if need[2] else None
-            if xr.numel():
-                nbytes = _C.query("vspw_group_norm_bwd_workspace", n, hw, c, groups, dt)
-                ws = _ws(nbytes, xr.device)
-                _C.call("vspw_group_norm_bwd", _p(xr), _p(gr), _p(dx), n, hw, c, groups, dt, _p(weight), _p(bias), act, p,
-                        _p(rng), channelwise, _p(stats), _p(dw), _p(db), _p(ws), nbytes, _stream())
-            else:
-                for t in (dw, db):
-                    if t is not None:
-                        t.zero_()
-        return (None if dx is None else dx.reshape(shape), dw, db) + (None,) * 6
+        return _norm_bwd(xr, g, weight, bias, rng, stats, ctx.meta, ctx.needs_input_grad) + (None,) * 6
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", p=0.0, rng=None, channelwise=False):
@@ -189,11 +233,17 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     if not eps >= 0.0:
         raise ValueError("group_norm_act: eps must not be negative, got %r" % eps)
     p = _check_rng("group_norm_act", p, rng)
+    if p == 0.0:
+        rng = None
     _same_device("group_norm_act", x, weight, bias, rng)
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and tuple(t.shape) != (c,):
-            raise RuntimeError("group_norm_act: %s must be [%d], got %s" % (name, c, tuple(t.shape)))
-    weight = None if weight is None else weight.float().contiguous()
-    bias = None if bias is None else bias.float().contiguous()
-    return GroupNormActFn.apply(x, weight, bias, num_groups, eps, _ACTS[act], p, rng if p > 0.0 else None,
-                                1 if channelwise else 0)
+    if weight is not None:
+        if weight.dim() != 1 or weight.shape[0] != c:
+            raise RuntimeError("group_norm_act: weight must be [%d], got %s" % (c, tuple(weight.shape)))
+        weight = weight.float().contiguous()
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != c:
+            raise RuntimeError("group_norm_act: bias must be [%d], got %s" % (c, tuple(bias.shape)))
+        bias = bias.float().contiguous()
+    if _wants_grad(x, weight, bias):
+        return GroupNormActFn.apply(x, weight, bias, num_groups, eps, _ACTS[act], p, rng, 1 if channelwise else 0)
+    return _norm_fwd(x, weight, bias, num_groups, eps, _ACTS[act], p, rng, 1 if channelwise else 0, False)[0]

@@ -196,6 +196,15 @@ __device__ __forceinline__ float half_max(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ int acc_index(int r, int lh) { return (r & 3) + 8 * (r >> 2) + 4 * lh; }
+// x - lam y as the same two roundings whether or not the maps are stored too
+__device__ __forceinline__ f32x4 da_mix(f32x4 x, f32x4 y, float lam) {
+#pragma clang fp contract(off)
+    return x - y * lam;
+}
+__device__ __forceinline__ f32x4 da_scaled(f32x4 x, float f) {
+#pragma clang fp contract(off)
+    return x * f;
+}
 __device__ __forceinline__ f32x4 quad(const f32x16& s, int g4) { return f32x4{s[4 * g4], s[4 * g4 + 1], s[4 * g4 + 2], s[4 * g4 + 3]}; }
 
 // A streamed [32][2D] tile on its way from global memory through registers into LDS: 16-byte vectors, thread t moves the
@@ -537,8 +546,8 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
             const int ch = 32 * j + 8 * g4 + 4 * lh;
-            const f32x4 x = quad(o1[j], g4) * i1, y = quad(o2[j], g4) * i2;
-            M::store4(out + ch, x - y * lam);
+            const f32x4 x = da_scaled(quad(o1[j], g4), i1), y = da_scaled(quad(o2[j], g4), i2);
+            M::store4(out + ch, da_mix(x, y, lam));
             if (a.maps) {
                 *reinterpret_cast<f32x4*>(a.maps + 2 * o + ch) = x;
                 *reinterpret_cast<f32x4*>(a.maps + 2 * o + W + ch) = y;
@@ -578,10 +587,10 @@ __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
         L1 = fmaf(v[1], w1, L1);
         L2 = fmaf(v[3], w2, L2);
     }
-    x *= L1 == 0.f ? 0.f : 1.f / L1;
-    y *= L2 == 0.f ? 0.f : 1.f / L2;
+    x = da_scaled(x, L1 == 0.f ? 0.f : 1.f / L1);
+    y = da_scaled(y, L2 == 0.f ? 0.f : 1.f / L2);
     const size_t o = (((size_t)(bh / a.hk) * a.nq + row / a.g) * a.h + head) * W + ch;
-    Mx<T>::store4(reinterpret_cast<T*>(a.out) + o, x - y * da_lambda(a, head));
+    Mx<T>::store4(reinterpret_cast<T*>(a.out) + o, da_mix(x, y, da_lambda(a, head)));
     if (a.maps) {
         *reinterpret_cast<f32x4*>(a.maps + 2 * (o - ch) + ch) = x;
         *reinterpret_cast<f32x4*>(a.maps + 2 * (o - ch) + W + ch) = y;
@@ -636,10 +645,10 @@ __global__ __launch_bounds__(256) void da_join_row_kernel(const DaArgs a) {
             x += sum[p * CT + tid];
             y += sum[p * CT + CT / 2 + tid];
         }
-        x *= L[0] == 0.f ? 0.f : 1.f / L[0];
-        y *= L[1] == 0.f ? 0.f : 1.f / L[1];
+        x = da_scaled(x, L[0] == 0.f ? 0.f : 1.f / L[0]);
+        y = da_scaled(y, L[1] == 0.f ? 0.f : 1.f / L[1]);
         const size_t o = (((size_t)(bh / a.hk) * a.nq + row / a.g) * a.h + head) * W;
-        Mx<T>::store4(reinterpret_cast<T*>(a.out) + o + 4 * tid, x - y * da_lambda(a, head));
+        Mx<T>::store4(reinterpret_cast<T*>(a.out) + o + 4 * tid, da_mix(x, y, da_lambda(a, head)));
         if (a.maps) {
             *reinterpret_cast<f32x4*>(a.maps + 2 * o + 4 * tid) = x;
             *reinterpret_cast<f32x4*>(a.maps + 2 * o + W + 4 * tid) = y;
@@ -1261,10 +1270,9 @@ static bool da_strides_ok(const vspw_dattn_desc* d, const DaPlan& p, const void*
     const long long s[] = {d->q_sb, d->q_sn, d->q_sh, d->q_sm, d->k_sb, d->k_sn, d->k_sh, d->k_sm, d->v_sb, d->v_sn, d->v_sh};
     for (long long x : s)
         if (x % ve) return false;
-    const long long near[] = {d->q_sn, d->q_sh, d->q_sm, d->k_sn, d->k_sm, d->v_sn};  // offsets inside a tile are 32 bits
+    const long long near[] = {d->q_sn, d->q_sm, d->k_sn, d->k_sm, d->v_sn, p.g > 1 ? p.g * d->q_sh : 0};  // inside a tile: 32 bits
     for (long long x : near)
         if (x < 0 || x >= DA_NEAR) return false;
-    if (p.g > 1 && (long long)p.g * d->q_sh >= 4 * DA_NEAR) return false;
     return (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0;
 }
 static void da_fill(DaArgs& a, const vspw_dattn_desc* d, const DaPlan& p, const void* q, const void* k, const void* v,

@@ -78,7 +78,9 @@ static int dropout_launch(const void* x, void* y, long long n, long long hw, int
     const bool aligned = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
     if (!channelwise) {
         const long long total = n * hw * c;
-        const dim3 grid(vspw_stream_grid((total + V - 1) / V, 256));
+        // one trip per thread up to 2^16 workgroups: 236 MB in and out at 5.7 TB/s, 1024 workgroups of many trips 5.2 TB/s
+        const long long trips = (total + V - 1) / V;
+        const dim3 grid((unsigned)(trips < (256LL << 16) ? (trips + 255) / 256 : 1 << 16));
         if (aligned)
             hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(256), 0, st, xp, yp, total, d, rng);
         else
@@ -86,7 +88,7 @@ static int dropout_launch(const void* x, void* y, long long n, long long hw, int
         return vspw_launch_status();
     }
     const bool vec = aligned && c % V == 0;
-    const SlabPlan s = vspw_slab_plan((int)n, hw, c, vec ? V : 1, 4);
+    const SlabPlan s = vspw_slab_plan((int)n, hw, c, vec ? V : 1, 4, 4096);
     const long long blocks = (long long)s.slabs * s.chunks * n;
     if (blocks > 0x7fffffffLL) return VSPW_EINVAL;
     if (vec)

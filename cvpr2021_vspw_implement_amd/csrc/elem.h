@@ -30,6 +30,21 @@ struct Vec<T, 1> {
     static __device__ __forceinline__ void store(T* p, const float* f) { p[0] = (T)f[0]; }
 };
 
+// V elements as one register value, unpacked when they are used.
+template <typename T, int V>
+struct Raw {
+    typedef T type __attribute__((ext_vector_type(V)));
+    static __device__ __forceinline__ void floats(const type& v, float* f) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = (float)v[e];
+    }
+};
+template <typename T>
+struct Raw<T, 1> {
+    typedef T type;
+    static __device__ __forceinline__ void floats(const type& v, float* f) { f[0] = (float)v; }
+};
+
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011): four independent
 // 32-bit words per 128-bit counter (ctr, offset) under the 64-bit key `seed`.  A word is a function of its index alone, so
 // forward and backward regenerate the same mask and nothing is stored.
@@ -102,7 +117,8 @@ static inline int vspw_dtype_size(int dtype) { return dtype == VSPW_F32 ? 4 : 2;
 struct SlabPlan {
     int v, tx, slabs, chunks;
 };
-static inline SlabPlan vspw_slab_plan(int n, long long hw, int c, int v, int min_trips) {
+// min_trips: pixels per thread that a workgroup is worth; blocks: how many workgroups fill the chip.
+static inline SlabPlan vspw_slab_plan(int n, long long hw, int c, int v, int min_trips, int blocks) {
     SlabPlan s;
     s.v = v;
     const int cv = (c + v - 1) / v;
@@ -110,7 +126,7 @@ static inline SlabPlan vspw_slab_plan(int n, long long hw, int c, int v, int min
     while (s.tx < cv && s.tx < 64) s.tx *= 2;
     s.slabs = (cv + s.tx - 1) / s.tx;
     const int ty = 256 / s.tx;
-    long long want = 1024 / ((long long)s.slabs * n);  // workgroups for 256 CUs x 4
+    long long want = blocks / ((long long)s.slabs * n);
     const long long most = (hw + (long long)ty * min_trips - 1) / ((long long)ty * min_trips);
     if (want > most) want = most;
     if (want < 1) want = 1;

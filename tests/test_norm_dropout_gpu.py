@@ -205,7 +205,10 @@ def norm_case(dev, shape, groups, dt, act="none", p=0.0, channelwise=False, affi
 @pytest.mark.parametrize("shape,groups", [
     ((2, 32, 8, 8), 4), ((1, 8, 1, 1), 1), ((3, 6, 5, 7), 3), ((2, 24, 3, 3), 8), ((2, 512, 6, 6), 32), ((1, 320, 4, 5), 20),
     ((2, 96, 7, 9), 32), ((1, 1056, 3, 4), 11), ((1, 16, 33, 31), 16), ((4, 64, 61, 3), 1), ((2, 65, 9, 4), 5),
-    ((3, 40, 17), 8), ((5, 48), 6), ((2, 16, 3, 5, 7), 4)])
+    ((3, 40, 17), 8), ((5, 48), 6), ((2, 16, 3, 5, 7), 4),
+    # images whose groups do not fit a workgroup's registers
+    ((2, 32, 40, 40), 4), ((1, 1056, 30, 31), 11), ((2, 65, 41, 39), 5), ((1, 3, 200, 190), 1), ((3, 2, 70, 60), 2),
+    ((1, 640, 23, 21), 2), ((2, 8, 9000), 4), ((1, 96, 1030), 32)])
 def test_group_norm_shapes(dev, dt, shape, groups):
     if shape == (1, 8, 1, 1):
         groups = 2
@@ -218,6 +221,8 @@ def test_group_norm_shapes(dev, dt, shape, groups):
 def test_group_norm_act_dropout(dev, dt, act, p, channelwise):
     norm_case(dev, (2, 48, 9, 11), 6, dt, act, p, channelwise)
     norm_case(dev, (2, 21, 5, 6), 7, dt, act, p, channelwise)  # 21 channels: the element-wise path
+    norm_case(dev, (2, 48, 41, 43), 6, dt, act, p, channelwise)  # streaming kernels
+    norm_case(dev, (1, 21, 41, 43), 7, dt, act, p, channelwise)
 
 
 @pytest.mark.parametrize("affine", [(True, False), (False, True), (False, False)])
@@ -229,6 +234,7 @@ def test_group_norm_layouts(dev):
     norm_case(dev, (2, 32, 6, 5), 8, "f32", layout="nchw")
     norm_case(dev, (2, 32, 6, 5), 8, "bf16", layout="nchw")
     norm_case(dev, (2, 32, 6, 5), 8, "bf16", layout="sliced")
+    norm_case(dev, (2, 32, 46, 45), 8, "bf16", layout="sliced")
 
 
 def test_group_norm_far_mean(dev):
