@@ -118,10 +118,10 @@ class ModelBuilder:
             net_decoder = PPMDeepsup_clip(num_class=num_class, fc_dim=fc_dim, use_softmax=use_softmax)
         elif arch == "ppm_clip":
             net_decoder = PPM_clip(num_class=num_class, fc_dim=fc_dim, use_softmax=use_softmax)
-        elif arch == "nonlocal2d":
+        elif arch in ("nonlocal2d", "nonlocal2d_differential"):
             from .non_local_models import Non_local2d
 
-            net_decoder = Non_local2d(num_class=num_class)
+            net_decoder = Non_local2d(num_class=num_class, nl_mode="dot" if arch == "nonlocal2d" else "differential")
         elif arch == "ocrnet_deepsup":
             from .ocrnet import SpatialOCRNet
 

@@ -23,6 +23,7 @@ from . import optim as voptim
 from .config import cfg
 from .dataset2 import BaseDataset, BaseDataset_longclip, DeviceTransform, collate_raw
 from .models import ModelBuilder, SegmentationModule
+from .models.non_local import NLBlockND
 from .train_clip2 import GraphedTrainStep, str2bool
 from .utils import AverageMeter, Evaluator, parse_devices, setup_logger
 
@@ -143,6 +144,10 @@ def group_weight(module):
                 no_decay.append(m.bias)
         elif isinstance(m, nn.modules.batchnorm._BatchNorm):
             no_decay.extend(p for p in (m.weight, m.bias) if p is not None)
+        elif isinstance(m, nn.GroupNorm):
+            no_decay.extend(p for p in (m.weight, m.bias) if p is not None)
+        elif isinstance(m, NLBlockND):  # the lambda vectors of mode 'differential'
+            no_decay.extend(m.parameters(recurse=False))
     assert len(list(module.parameters())) == len(decay) + len(no_decay)
     return [dict(params=decay), dict(params=no_decay, weight_decay=.0)]
 

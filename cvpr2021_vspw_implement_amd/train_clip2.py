@@ -415,6 +415,8 @@ def build_parser():
                    help="replay the training step as one captured hipGraph (fixed crop / batch shapes; no reference "
                         "counterpart)")
     p.add_argument("--raft_weights", type=str, default="./RAFT_core/raft-things.pth-no-zip")
+    p.add_argument("--nl_mode", default="dot", choices=["dot", "differential"],
+                   help="affinity of the nonlocal3d block: the reference's dot product or the difference of two softmax maps")
     p.add_argument("opts", help="Modify config options using the command-line", default=None, nargs=argparse.REMAINDER)
     return p
 

@@ -1,0 +1,158 @@
+"""The non-local block in mode 'differential' - attention, head normalisation, dropout, projection, residual in one run -
+against the same chain in float64 on the CPU, and the decoders that own it.
+
+Tolerance of the chain: every stage (five projections / products of up to 256 terms, two softmax, two normalisations) adds a
+relative error of a few 2^-24 sqrt(256) = 1e-6; 5e-5 of the norm leaves a factor of five to the amplification of the two
+normalisations' backward passes."""
+import math
+
+import pytest
+import torch
+from test_norm_dropout_gpu import keep64
+
+pytestmark = pytest.mark.gpu
+REL = 5e-5
+
+
+def block64(m, x, seed, train, go):
+    """z, dx and parameter gradients of NLBlockND(mode='differential') in float64, from its definition."""
+    P = {k: v.detach().double().cpu().requires_grad_(True) for k, v in m.named_parameters()}
+    x = x.detach().double().cpu().requires_grad_(True)
+    b, c = x.shape[:2]
+    n = x[0, 0].numel()
+    h, ci = m.heads, m.inter_channels
+    d = ci // (2 * h)
+    xr = x.reshape(b, c, n)
+
+    def conv(name, t):
+        return torch.einsum("oc,bcn->bon", P[name + ".weight"].reshape(-1, t.shape[1]), t) + P[name + ".bias"][None, :, None]
+
+    q = conv("theta", xr).reshape(b, h, 2, d, n)
+    k = conv("phi", xr).reshape(b, h, 2, d, n)
+    v = conv("g", xr).reshape(b, h, 2 * d, n)
+    lam = (torch.exp((P["lambda_q1"] * P["lambda_k1"]).sum(1)) - torch.exp((P["lambda_q2"] * P["lambda_k2"]).sum(1))
+           + m.lambda_init)
+    s = torch.einsum("bhmdi,bhmdj->bhmij", q, k) / math.sqrt(d)
+    if m.frame_causal:
+        f = n // x.shape[2]
+        i, j = torch.arange(n)[:, None] // f, torch.arange(n)[None, :] // f
+        s = s.masked_fill(j > i, -math.inf)
+    p = torch.softmax(s, -1)
+    y = torch.einsum("bhij,bhdj->bhdi", p[:, :, 0] - lam[None, :, None, None] * p[:, :, 1], v)
+    yg = y.reshape(b, h, -1)
+    mu = yg.mean(2, keepdim=True)
+    yg = (yg - mu) / torch.sqrt(((yg - mu) ** 2).mean(2, keepdim=True) + m.norm.eps)
+    y = yg.reshape(b, ci, n) * P["norm.weight"][None, :, None] + P["norm.bias"][None, :, None]
+    if train and m.drop.p > 0:
+        y = y * keep64((b, ci, n), m.drop.p, torch.tensor([seed, 0]), False)
+    z = conv("W_z.0", y)
+    bn = m.W_z[1]
+    if train:
+        mean, var = z.mean((0, 2), keepdim=True), z.var((0, 2), unbiased=False, keepdim=True)
+    else:
+        mean, var = (t.detach().double().cpu()[None, :, None] for t in (bn.running_mean, bn.running_var))
+    z = (z - mean) / torch.sqrt(var + bn.eps) * P["W_z.1.weight"][None, :, None] + P["W_z.1.bias"][None, :, None] + xr
+    z = z.reshape(x.shape)
+    z.backward(go.double().cpu())
+    return z.detach(), x.grad, {k: t.grad for k, t in P.items()}
+
+
+def close(a, b, what, floor=0.0):
+    a, b = a.detach().double().cpu(), b.double().cpu()
+    assert a.shape == b.shape, what
+    err = (a - b).norm().item()
+    assert err <= REL * b.norm().item() + floor, "%s: %.3e of %.3e" % (what, err, b.norm())
+
+
+def make_block(dev, **kw):
+    from cvpr2021_vspw_implement_amd.models.non_local import NLBlockND
+
+    torch.manual_seed(7)
+    m = NLBlockND(in_channels=64, mode="differential", **kw).to(dev)
+    torch.nn.init.normal_(m.W_z[1].weight, 1.0, 0.1)
+    torch.nn.init.normal_(m.W_z[1].bias, 0.0, 0.1)
+    return m
+
+
+@pytest.mark.parametrize("kw,shape", [
+    (dict(inter_channels=64, dimension=2, heads=2), (2, 64, 9, 11)),
+    (dict(inter_channels=128, dimension=2, heads=1, dropout=0.2), (1, 64, 13, 7)),
+    (dict(inter_channels=64, dimension=3, heads=1, dropout=0.1), (2, 64, 3, 6, 5)),
+    (dict(inter_channels=128, dimension=3, heads=4, frame_causal=True), (1, 64, 4, 7, 6)),
+])
+@pytest.mark.parametrize("train", [True, False])
+def test_block(dev, kw, shape, train):
+    m = make_block(dev, **kw).train(train)
+    m.drop.manual_seed(91)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(shape, generator=g).to(dev).requires_grad_(True)
+    go = torch.randn(shape, generator=g).to(dev)
+    z = m(x)
+    z.backward(go)
+    rz, rx, rp = block64(m, x, 91, train, go)
+    close(z, rz, "z")
+    close(x.grad, rx, "dx")
+    scale = max(t.norm().item() for t in rp.values())
+    for k, p in m.named_parameters():
+        # a bias in front of a normalisation has a zero gradient: what is left is rounding of the largest one
+        close(p.grad, rp[k], k, floor=REL * scale * (1.0 if k in ("W_z.0.bias", "phi.bias") else 0.02))
+
+
+def test_captured_block_replays_with_new_masks(dev):
+    """Forward and backward of the block as one graph: every replay equals the eager step with the same generator offset."""
+    m = make_block(dev, inter_channels=64, dimension=2, heads=2, dropout=0.3).train()
+    m.W_z[1].momentum = 0.0
+    x = torch.randn(2, 64, 8, 9, device=dev).contiguous(memory_format=torch.channels_last)
+    go = torch.randn_like(x)
+    params = [p for p in m.parameters()]
+
+    def step():
+        leaf = x.detach().requires_grad_(True)
+        z = m(leaf)
+        return (z.detach(),) + torch.autograd.grad(z, [leaf] + params, go)
+
+    m.drop.manual_seed(4)
+    eager = [[t.clone() for t in step()] for _ in range(3)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    m.drop.manual_seed(4)
+    for i in range(3):
+        graph.replay()
+        m.norm.weight.sum()  # eager work between the replays
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager[i])), i
+
+
+def test_decoders(dev):
+    """The per-frame decoder and the clip head with the differential block: one training step and inference run."""
+    import cvpr2021_vspw_implement_amd.models as M
+    from helpers import args_ns
+
+    torch.manual_seed(2)
+    dec = M.ModelBuilder.build_decoder(arch="nonlocal2d_differential", fc_dim=2048, num_class=12).to(dev)
+    feat = torch.randn(2, 2048, 9, 10, device=dev)
+    out = dec([feat])
+    assert out.shape == (2, 12, 9, 10)
+    out.sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in dec.parameters())
+    with torch.no_grad():
+        probs = dec.eval()([feat], segSize=(18, 20))
+    assert probs.shape == (2, 12, 18, 20) and (probs.sum(1) - 1).abs().max() < 1e-5
+
+    class Enc(torch.nn.Module):
+        def forward(self, x, return_feature_maps=False):
+            return [x]
+
+    crit = torch.nn.NLLLoss(ignore_index=255)
+    head = M.Non_local3d(args_ns(num_class=12, nl_mode="differential"), Enc(), crit).to(dev)
+    clip = [torch.randn(1, 2048, 6, 7, device=dev) for _ in range(3)]
+    labs = [torch.randint(0, 12, (1, 1, 48, 56), device=dev).float() for _ in range(3)]
+    loss, _ = head({"clipimgs_data": clip, "cliplabels_data": labs})
+    loss.backward()
+    assert torch.isfinite(loss) and all(torch.isfinite(p.grad).all() for p in head.parameters())
