@@ -86,6 +86,9 @@ struct Mx<float> {
     static __device__ __forceinline__ void step(f32x16& acc, const Frag& x, const Frag& y, int e) {
         acc = __builtin_amdgcn_mfma_f32_32x32x2f32(e < 4 ? x.a[e & 3] : x.b[e & 3], e < 4 ? y.a[e & 3] : y.b[e & 3], acc, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x16 first(const Frag& x, const Frag& y, const f32x16& c) {  // step 0 onto c
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(x.a[0], y.a[0], c, 0, 0, 0);
+    }
     static __device__ __forceinline__ void rstep(f32x16& acc, const Frag& x, const RegFrag& y, int e) { step(acc, x, y, e); }
     static __device__ __forceinline__ void store4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
 };
@@ -137,6 +140,9 @@ struct Mx<bf16_t> {
     }
     static __device__ __forceinline__ void step(f32x16& acc, const Frag& x, const Frag& y, int) {
         acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 first(const Frag& x, const Frag& y, const f32x16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
     }
     static __device__ __forceinline__ void rstep(f32x16& acc, const Frag& x, const RegFrag& y, int e) {
         acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, e ? y.lo : y.hi, acc, 0, 0, 0);
@@ -235,20 +241,21 @@ template <typename T, int D, int THREADS>
 struct KeyStream {
     typedef Stager<T, D, THREADS> St;
     St k, v;
-    const char *kb, *vb;
+    const char *kp, *vp;      // the next tile to fetch; the last one of the tensor is fetched again and again
     const unsigned char* mb;  // the mask's row, or any readable byte when there is none
     long long ks, vs;         // bytes from key to key
     unsigned k0, v0, kc, vc;  // this thread's first row and column in bytes
     unsigned live1, live2;    // which keys of the last two tiles of k take part
-    int begin, end, nk, ktile, mstep, open;
+    int begin, end, nk, krem, vrem, ktile, mstep, open;  // ?rem: keys of the tensor behind the first of the next tile
     unsigned char raw;
 
     __device__ __forceinline__ void init(const DaArgs& a, int tid, int bi, int kh, int part, int last_row) {
         constexpr int E = (int)sizeof(T);
-        kb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + bi * a.k_sb + kh * a.k_sh);
-        vb = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + bi * a.v_sb + kh * a.v_sh);
+        begin = part * a.span;  // below nk
+        kp = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + bi * a.k_sb + kh * a.k_sh + begin * a.k_sn);
+        vp = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + bi * a.v_sb + kh * a.v_sh + begin * a.v_sn);
         open = a.mask == nullptr;
-        mb = open ? reinterpret_cast<const unsigned char*>(kb) : a.mask + (size_t)bi * a.nk;
+        mb = open ? reinterpret_cast<const unsigned char*>(kp) : a.mask + (size_t)bi * a.nk;
         mstep = open ? 0 : 1;
         ks = a.k_sn * E;
         vs = a.v_sn * E;
@@ -258,7 +265,8 @@ struct KeyStream {
         kc = (c >= D ? (unsigned)a.k_sm + c - D : c) * E;
         vc = c * E;
         nk = a.nk;
-        begin = part * a.span;
+        krem = vrem = nk - 1 - begin;
+        ktile = begin - DA_TILE;
         end = min(min(a.nk, begin + a.span), da_limit(a, last_row));
         live1 = live2 = 0;
     }
@@ -267,18 +275,24 @@ struct KeyStream {
     __device__ __forceinline__ int plain(const DaArgs& a, int first_row) const {
         return a.frame ? max(0, da_limit(a, first_row) - begin) / DA_TILE : tiles();
     }
-    // vector i of tile t; tiles past the end read the last key again
-    __device__ __forceinline__ void get_k(int tid, int i, int t) {
-        const int key0 = min(begin + t * DA_TILE, nk - 1);
-        k.get(i, kb + key0 * ks, min(k0 + i * St::STEP * (unsigned)ks, min(nk - 1 - key0, DA_TILE) * (unsigned)ks) + kc);
+    // vector i of the next tile; the last vector moves on
+    __device__ __forceinline__ void get_k(int tid, int i) {
         if (i == 0) {
-            ktile = begin + t * DA_TILE;
-            raw = mb[(size_t)min(ktile + tid % DA_TILE, nk - 1) * mstep];
+            ktile += DA_TILE;
+            raw = mb[(unsigned)(min(ktile + tid % DA_TILE, nk - 1) * mstep)];
+        }
+        k.get(i, kp, min(k0 + i * St::STEP * (unsigned)ks, (unsigned)min(krem, DA_TILE) * (unsigned)ks) + kc);
+        if (i == St::F - 1) {
+            kp += krem >= DA_TILE ? DA_TILE * ks : 0;
+            krem -= krem >= DA_TILE ? DA_TILE : 0;
         }
     }
-    __device__ __forceinline__ void get_v(int i, int t) {
-        const int key0 = min(begin + t * DA_TILE, nk - 1);
-        v.get(i, vb + key0 * vs, min(v0 + i * St::STEP * (unsigned)vs, min(nk - 1 - key0, DA_TILE) * (unsigned)vs) + vc);
+    __device__ __forceinline__ void get_v(int i) {
+        v.get(i, vp, min(v0 + i * St::STEP * (unsigned)vs, (unsigned)min(vrem, DA_TILE) * (unsigned)vs) + vc);
+        if (i == St::F - 1) {
+            vp += vrem >= DA_TILE ? DA_TILE * vs : 0;
+            vrem -= vrem >= DA_TILE ? DA_TILE : 0;
+        }
     }
     __device__ __forceinline__ void put_k(int tid, int i, T* K, float* B) {
         if (i == 0) {
@@ -359,6 +373,7 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
     for (int j = 0; j < CB; ++j) o1[j] = o2[j] = zero16();
     float m1 = -DA_INF, m2 = -DA_INF, l1 = 0.f, l2 = 0.f, x1 = -DA_INF, x2 = -DA_INF;
     Frag ga, gb;  // the first operands of the next A
+    f32x16 bias;
 
     // one entry of both maps' scores of the tile at key0: later frames to -inf (EDGE), running maximum
     auto entry = [&](auto edge, f32x16& u, f32x16& w, int r, int key0) {
@@ -375,11 +390,12 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
         x2 = half_max(x2) * a.c;
     };
     auto ready = [&](int buf) {  // what the next A starts from
-        n1 = n2 = da_bias(Kb[buf], lh);
+        bias = da_bias(Kb[buf], lh);
         ga = M::row(Ks[buf] + l31 * LD, lh);
         gb = M::row(Ks[buf] + l31 * LD + D, lh);
     };
-    auto body = [&](auto next, auto edge, int t) {
+    // one tile: its scores in (s1, s2), those of the next left in (n1, n2); two calls in turn save the copy (bf16: 8 %)
+    auto body = [&](auto next, auto edge, int t, f32x16& s1, f32x16& s2, f32x16& n1, f32x16& n2) {
         constexpr bool NEXT = decltype(next)::value;
         const int cur = t & 1, nxt = cur ^ 1, key1 = ks.begin + (t + 1) * DA_TILE;
         // The sums are rescaled only when a maximum has grown by more than 2^8: weights stay below 256.
@@ -410,7 +426,10 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
             }
 #pragma unroll
             for (int e = 0; e < M::STEPS; ++e) {
-                if (NEXT) {
+                if (NEXT && i + e == 0) {
+                    n1 = M::first(fa, q1[0], bias);
+                    n2 = M::first(fb, q2[0], bias);
+                } else if (NEXT) {
                     M::step(n1, fa, q1[i], e);
                     M::step(n2, fb, q2[i], e);
                 }
@@ -430,7 +449,7 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
 #pragma unroll
                     for (int f = slot * St::F / SL; f < (slot + 1) * St::F / SL; ++f) {
                         ks.put_k(tid, f, Ks[cur], Kb[cur]);
-                        ks.get_k(tid, f, t + 3);
+                        ks.get_k(tid, f);
                     }
                 }
                 da_pin();
@@ -461,7 +480,7 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
 #pragma unroll
                         for (int f = slot * St::F / SB; f < (slot + 1) * St::F / SB; ++f) {
                             ks.put_v(tid, f, Vs[nxt], ks.live1);
-                            ks.get_v(f, t + 2);
+                            ks.get_v(f);
                         }
                     }
                     da_pin();
@@ -469,8 +488,6 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
             }
         }
         if (NEXT) {
-            s1 = n1;
-            s2 = n2;
             finish_max();
             ready(cur);
         }
@@ -479,17 +496,17 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
     if (ntiles > 0) {
 #pragma unroll
         for (int f = 0; f < St::F; ++f) {
-            ks.get_k(tid, f, 0);
-            ks.get_v(f, 0);
+            ks.get_k(tid, f);
+            ks.get_v(f);
         }
 #pragma unroll
         for (int f = 0; f < St::F; ++f) {
             ks.put_k(tid, f, Ks[0], Kb[0]);
             ks.put_v(tid, f, Vs[0], ks.live2);
-            ks.get_v(f, 1);
+            ks.get_v(f);
         }
 #pragma unroll
-        for (int f = 0; f < St::F; ++f) ks.get_k(tid, f, 1);
+        for (int f = 0; f < St::F; ++f) ks.get_k(tid, f);
         __syncthreads();
         s1 = s2 = da_bias(Kb[0], lh);
         const T* K0 = Ks[0] + l31 * LD;
@@ -508,17 +525,28 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
 #pragma unroll
         for (int f = 0; f < St::F; ++f) {
             ks.put_k(tid, f, Ks[1], Kb[1]);
-            ks.get_k(tid, f, 2);
+            ks.get_k(tid, f);
         }
         __syncthreads();
         ready(1);
         int t = 0;
         if (M::ONE_LOOP) {
-            for (; t < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+            for (; t < ntiles; ++t) {  // the tile past the end has weights 0
+                body(DA_BOOL(true), DA_BOOL(true), t, s1, s2, n1, n2);
+                s1 = n1;
+                s2 = n2;
+            }
         } else {  // tiles that every row of the workgroup sees whole come first
-            for (; t + 1 < min(nplain, ntiles); ++t) body(DA_BOOL(true), DA_BOOL(false), t);
-            for (; t + 1 < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
-            body(DA_BOOL(false), DA_BOOL(false), t);
+            for (; t + 2 < min(nplain, ntiles); t += 2) {
+                body(DA_BOOL(true), DA_BOOL(false), t, s1, s2, n1, n2);
+                body(DA_BOOL(true), DA_BOOL(false), t + 1, n1, n2, s1, s2);
+            }
+            for (; t + 1 < ntiles; ++t) {
+                body(DA_BOOL(true), DA_BOOL(true), t, s1, s2, n1, n2);
+                s1 = n1;
+                s2 = n2;
+            }
+            body(DA_BOOL(false), DA_BOOL(false), t, s1, s2, n1, n2);
         }
     }
     l1 += __shfl_xor(l1, 32, 64);
@@ -760,16 +788,16 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
 #pragma unroll
     for (int j = 0; j < DB; ++j) g1[j] = g2[j] = zero16();
     Frag ga, gb, gc, gd;  // the first operands of the next A
+    f32x16 bias;
 
     auto ready = [&](int kbuf, int vbuf) {
-        n1 = n2 = da_bias(Kb[kbuf], lh);
-        np = zero16();
+        bias = da_bias(Kb[kbuf], lh);
         ga = M::row(Ks[kbuf] + l31 * LD, lh);
         gb = M::row(Ks[kbuf] + l31 * LD + D, lh);
         gc = M::row(Vs[vbuf] + l31 * LD, lh);
         gd = M::row(Vs[vbuf] + l31 * LD + 16, lh);
     };
-    auto body = [&](auto next, auto edge, int t) {
+    auto body = [&](auto next, auto edge, int t, f32x16& s1, f32x16& s2, f32x16& dp, f32x16& n1, f32x16& n2, f32x16& np) {
         constexpr bool NEXT = decltype(next)::value;
         const int key0 = ks.begin + t * DA_TILE, b0 = t & 3, b2 = (t + 2) & 3;
         const T *Kn = Ks[(t + 1) & 3] + l31 * LD, *Vn = Vs[(t + 1) & 1] + l31 * LD;
@@ -785,7 +813,12 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
             }
 #pragma unroll
             for (int e = 0; e < M::STEPS; ++e) {
-                if (NEXT) {
+                if (NEXT && i + e == 0) {
+                    n1 = M::first(fa, q1[0], bias);
+                    np = M::first(fc, go[0], zero16());
+                    n2 = M::first(fb, q2[0], bias);
+                    M::step(np, fd, go[1], 0);
+                } else if (NEXT) {
                     M::step(n1, fa, q1[i], e);
                     M::step(np, fc, go[2 * i], e);
                     M::step(n2, fb, q2[i], e);
@@ -804,8 +837,8 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
                     for (int f = slot * St::F / SL; f < (slot + 1) * St::F / SL; ++f) {
                         ks.put_k(tid, f, Ks[b2], Kb[b2]);
                         ks.put_v(tid, f, Vs[t & 1], ks.live2);
-                        ks.get_k(tid, f, t + 3);
-                        ks.get_v(f, t + 3);
+                        ks.get_k(tid, f);
+                        ks.get_v(f);
                     }
                 }
                 da_pin();
@@ -833,19 +866,14 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
                 da_pin();
             }
         }
-        if (NEXT) {
-            s1 = n1;
-            s2 = n2;
-            dp = np;
-            ready(b2, t & 1);
-        }
+        if (NEXT) ready(b2, t & 1);
     };
 
     if (ntiles > 0) {
 #pragma unroll
         for (int f = 0; f < St::F; ++f) {
-            ks.get_k(tid, f, 0);
-            ks.get_v(f, 0);
+            ks.get_k(tid, f);
+            ks.get_v(f);
         }
 #pragma unroll
         for (int f = 0; f < St::F; ++f) {
@@ -854,8 +882,8 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
         }
 #pragma unroll
         for (int f = 0; f < St::F; ++f) {
-            ks.get_k(tid, f, 1);
-            ks.get_v(f, 1);
+            ks.get_k(tid, f);
+            ks.get_v(f);
         }
         __syncthreads();
         s1 = s2 = da_bias(Kb[0], lh);
@@ -876,18 +904,31 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
         for (int f = 0; f < St::F; ++f) {
             ks.put_k(tid, f, Ks[1], Kb[1]);
             ks.put_v(tid, f, Vs[1], ks.live2);
-            ks.get_k(tid, f, 2);
-            ks.get_v(f, 2);
+            ks.get_k(tid, f);
+            ks.get_v(f);
         }
         __syncthreads();
         ready(1, 1);
         int t = 0;
         if (M::ONE_LOOP) {
-            for (; t < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+            for (; t < ntiles; ++t) {
+                body(DA_BOOL(true), DA_BOOL(true), t, s1, s2, dp, n1, n2, np);
+                s1 = n1;
+                s2 = n2;
+                dp = np;
+            }
         } else {
-            for (; t < min(nplain, ntiles - 1); ++t) body(DA_BOOL(true), DA_BOOL(false), t);
-            for (; t + 1 < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
-            body(DA_BOOL(false), DA_BOOL(true), t);
+            for (; t + 1 < min(nplain, ntiles - 1); t += 2) {
+                body(DA_BOOL(true), DA_BOOL(false), t, s1, s2, dp, n1, n2, np);
+                body(DA_BOOL(true), DA_BOOL(false), t + 1, n1, n2, np, s1, s2, dp);
+            }
+            for (; t + 1 < ntiles; ++t) {
+                body(DA_BOOL(true), DA_BOOL(true), t, s1, s2, dp, n1, n2, np);
+                s1 = n1;
+                s2 = n2;
+                dp = np;
+            }
+            body(DA_BOOL(false), DA_BOOL(true), t, s1, s2, dp, n1, n2, np);
         }
     }
     if (!ro.live) return;
@@ -994,13 +1035,12 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     Frag ga, gb_, gc, gd;  // the first operands of the next A
 
     auto ready = [&](int buf) {
-        n1 = n2 = np = zero16();
         ga = M::row(Qs[buf] + l31 * LD, lh);
         gb_ = M::row(Qs[buf] + l31 * LD + D, lh);
         gc = M::row(Gs[buf] + l31 * LD, lh);
         gd = M::row(Gs[buf] + l31 * LD + 16, lh);
     };
-    auto body = [&](auto next, auto edge, int t) {
+    auto body = [&](auto next, auto edge, int t, f32x16& s1, f32x16& s2, f32x16& dp, f32x16& n1, f32x16& n2, f32x16& np) {
         constexpr bool NEXT = decltype(next)::value;
         const int b0 = t & 3, b1 = (t + 1) & 3, b2 = (t + 2) & 3;
         const T *Qn = Qs[b1] + l31 * LD, *Gn = Gs[b1] + l31 * LD;
@@ -1018,7 +1058,12 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
             }
 #pragma unroll
             for (int e = 0; e < M::STEPS; ++e) {
-                if (NEXT) {
+                if (NEXT && i + e == 0) {
+                    n1 = M::first(fa, k1[0], zero16());
+                    np = M::first(fc, v[0], zero16());
+                    n2 = M::first(fb, k2[0], zero16());
+                    M::step(np, fd, v[1], 0);
+                } else if (NEXT) {
                     M::step(n1, fa, k1[i], e);
                     M::step(np, fc, v[2 * i], e);
                     M::step(n2, fb, k2[i], e);
@@ -1086,12 +1131,7 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
                 da_pin();
             }
         }
-        if (NEXT) {
-            s1 = n1;
-            s2 = n2;
-            dp = np;
-            ready(b2);
-        }
+        if (NEXT) ready(b2);
     };
 
     if (ntiles > 0) {
@@ -1125,11 +1165,31 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
         ready(1);
         int t = 0;
         if (M::ONE_LOOP) {
-            for (; t < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(true), t);
+            for (; t < ntiles; ++t) {
+                body(DA_BOOL(true), DA_BOOL(true), t, s1, s2, dp, n1, n2, np);
+                s1 = n1;
+                s2 = n2;
+                dp = np;
+            }
         } else {
-            for (; t < min(nedge, ntiles - 1); ++t) body(DA_BOOL(true), DA_BOOL(true), t);
-            for (; t + 1 < ntiles; ++t) body(DA_BOOL(true), DA_BOOL(false), t);
-            body(DA_BOOL(false), DA_BOOL(true), t);
+            for (; t < min(nedge, ntiles - 1); ++t) {
+                body(DA_BOOL(true), DA_BOOL(true), t, s1, s2, dp, n1, n2, np);
+                s1 = n1;
+                s2 = n2;
+                dp = np;
+            }
+            for (; t + 2 < ntiles; t += 2) {
+                body(DA_BOOL(true), DA_BOOL(false), t, s1, s2, dp, n1, n2, np);
+                body(DA_BOOL(true), DA_BOOL(false), t + 1, n1, n2, np, s1, s2, dp);
+            }
+            if (t + 1 < ntiles) {
+                body(DA_BOOL(true), DA_BOOL(true), t, s1, s2, dp, n1, n2, np);
+                s1 = n1;
+                s2 = n2;
+                dp = np;
+                ++t;
+            }
+            body(DA_BOOL(false), DA_BOOL(true), t, s1, s2, dp, n1, n2, np);
         }
     }
     if (key >= a.nk) return;
