@@ -201,10 +201,12 @@ def _norm_bwd(xr, g, weight, bias, rng, stats, meta, need):
 
 
 class GroupNormActFn(torch.autograd.Function):
-    """y = dropout(act(group_norm(x))); the backward pass re-reads x and the fp64 statistics [N,groups,2]."""
+    """y = dropout(act(group_norm(x))); the backward pass re-reads x and the fp64 statistics [N,groups,2].
+    how: (groups, eps, act, p, channelwise)."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, p, rng, channelwise):
+    def forward(ctx, x, weight, bias, rng, how):
+        groups, eps, act, p, channelwise = how
         y, xr, stats = _norm_fwd(x, weight, bias, groups, eps, act, p, rng, channelwise, True)
         ctx.meta = (groups, act, p, channelwise, x.shape)
         ctx.save_for_backward(xr, weight, bias, rng, stats)
@@ -213,7 +215,7 @@ class GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         xr, weight, bias, rng, stats = ctx.saved_tensors
-        return _norm_bwd(xr, g, weight, bias, rng, stats, ctx.meta, ctx.needs_input_grad) + (None,) * 6
+        return _norm_bwd(xr, g, weight, bias, rng, stats, ctx.meta, ctx.needs_input_grad) + (None, None)
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", p=0.0, rng=None, channelwise=False):
@@ -245,5 +247,5 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
             raise RuntimeError("group_norm_act: bias must be [%d], got %s" % (c, tuple(bias.shape)))
         bias = bias.float().contiguous()
     if _wants_grad(x, weight, bias):
-        return GroupNormActFn.apply(x, weight, bias, num_groups, eps, _ACTS[act], p, rng, 1 if channelwise else 0)
+        return GroupNormActFn.apply(x, weight, bias, rng, (num_groups, eps, _ACTS[act], p, 1 if channelwise else 0))
     return _norm_fwd(x, weight, bias, num_groups, eps, _ACTS[act], p, rng, 1 if channelwise else 0, False)[0]

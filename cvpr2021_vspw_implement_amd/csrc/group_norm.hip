@@ -8,7 +8,7 @@
 // from zero costs no digits.  The mean enters the fp32 arithmetic as two terms; ReLU's border is decided on the fp64
 // pre-activation (the same in both directions).  All sums have a fixed order: results are bit-reproducible.
 //
-// Large images: streaming kernels, stats -> apply and bwd_stats -> bwd_reduce -> bwd_apply, bound by HBM.  Images whose
+// Large images: streaming kernels, stats -> finish -> apply and bwd_stats -> bwd_reduce -> bwd_apply, bound by HBM.  Images whose
 // groups fit the registers of a workgroup: one workgroup per image and group, which reads its elements once.
 #include <type_traits>
 
@@ -20,7 +20,8 @@ struct GnShape {
     long long hw;
     int n, c, groups, cpg;  // cpg: channels per group
     int tx, slabs, chunks;  // streaming kernels
-    int fx, trips;          // one workgroup per image and group: vectors per pixel of a group, pixels per thread (0: does not fit)
+    int fx;                 // vectors per pixel of a group
+    bool group;             // one workgroup per image and group
 };
 // Where a streaming workgroup stands.
 struct GnPlace {
@@ -97,10 +98,10 @@ __device__ __forceinline__ void reduce_pixels(double* s, double* q, double (*red
     }
 }
 
-// Calls run(p, 4) for four pixels at a time and run(p, 1) for the rest, so that four loads are in flight.
-template <typename F>
+// Calls run(p, U) for U pixels at a time and run(p, 1) for the rest, so that U loads of every tensor are in flight.
+template <int U, typename F>
 __device__ __forceinline__ void walk(long long p, long long step, long long hw, F run) {
-    for (; p + 3 * step < hw; p += 4 * step) run(p, std::integral_constant<int, 4>());
+    for (; p + (U - 1) * step < hw; p += U * step) run(p, std::integral_constant<int, U>());
     for (; p < hw; p += step) run(p, std::integral_constant<int, 1>());
 }
 
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, 
 #pragma unroll
         for (int e = 0; e < V; ++e) x0[e] = (float)xi[(c0 + e) / g.cpg * g.cpg];
         const long long step = (long long)g.chunks * ty;
-        walk((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
+        walk<4>((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
             constexpr int N = decltype(nn)::value;
             float f[N][V];
 #pragma unroll
@@ -156,43 +157,32 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const T* __restrict__ x, 
     }
 }
 
-// mean and 1/sqrt(var + eps) of the groups that overlap the block's slab, into LDS ms[k][2]: entries of all chunks and of
-// the slabs that share the group, summed in a fixed order by `lanes` lanes per group.
+// stats[img][group] = mean, 1/sqrt(var + eps): one wave per image and group sums the entries of all chunks and of the slabs
+// that share the group, in a fixed order.  (Every workgroup of the apply kernel doing it for itself read 0.5 GB of partial
+// sums at [4,256,119,119]: 32 us where this and the bare apply kernel take 20.)
 template <typename T>
-__device__ __forceinline__ void group_stats(const T* __restrict__ x, const double* __restrict__ part, const GnShape& g,
-                                            int gs, int img, int slab, int slabw, float eps, double* ms) {
-    const int first = slab * slabw, last = min(g.c, first + slabw);
-    const int g0 = first / g.cpg, count = (last - 1) / g.cpg - g0 + 1;
-    int lanes = 64;
-    while (lanes > 1 && 256 / lanes < count) lanes >>= 1;
-    const int sub = threadIdx.x % lanes;
-    const double inv = 1.0 / ((double)g.hw * g.cpg);
-    for (int k0 = 0; k0 < count; k0 += 256 / lanes) {
-        const int k = k0 + threadIdx.x / lanes;
-        double a = 0, b = 0;
-        if (k < count) {
-            const int gr = g0 + k;
-            const int s0 = gr * g.cpg / slabw, ns = ((gr + 1) * g.cpg - 1) / slabw - s0 + 1;
-            for (int i = sub; i < g.chunks * ns; i += lanes) {
-                const int sl = s0 + i % ns;
-                const double* o = part + ((((size_t)img * g.chunks + i / ns) * g.slabs + sl) * gs + (gr - sl * slabw / g.cpg)) * 2;
-                a += o[0];
-                b += o[1];
-            }
-        }
-        for (int o = lanes >> 1; o > 0; o >>= 1) {
-            a += __shfl_xor(a, o, 64);
-            b += __shfl_xor(b, o, 64);
-        }
-        if (k < count && sub == 0) {
-            const double m = a * inv;
-            double var = b * inv - m * m;
-            if (var < 0) var = 0;
-            ms[2 * k] = m + (double)(float)x[(size_t)img * g.hw * g.c + (size_t)(g0 + k) * g.cpg];
-            ms[2 * k + 1] = 1.0 / sqrt(var + (double)eps);
-        }
+__global__ __launch_bounds__(256) void gn_finish_kernel(const T* __restrict__ x, const double* __restrict__ part, GnShape g,
+                                                        int gs, int slabw, float eps, double* __restrict__ stats) {
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (long long)g.n * g.groups) return;
+    const int img = (int)(id / g.groups), gr = (int)(id % g.groups), lane = threadIdx.x & 63;
+    const int s0 = gr * g.cpg / slabw, ns = ((gr + 1) * g.cpg - 1) / slabw - s0 + 1;
+    double a = 0, b = 0;
+#pragma unroll 4
+    for (int i = lane; i < g.chunks * ns; i += 64) {
+        const int sl = s0 + i % ns;
+        const double* o = part + ((((size_t)img * g.chunks + i / ns) * g.slabs + sl) * gs + (gr - sl * slabw / g.cpg)) * 2;
+        a += o[0];
+        b += o[1];
     }
-    __syncthreads();
+    a = wave_sum_d(a);
+    b = wave_sum_d(b);
+    if (lane == 0) {
+        const double inv = 1.0 / ((double)g.hw * g.cpg), m = a * inv;
+        const double var = b * inv - m * m;
+        stats[2 * id] = m + (double)(float)x[(size_t)img * g.hw * g.c + (size_t)gr * g.cpg];
+        stats[2 * id + 1] = 1.0 / sqrt((var < 0 ? 0 : var) + (double)eps);
+    }
 }
 
 // The dropout factors of one pixel's channels c0 .. c0+V-1 (memory index e0); ck: the channel form's, computed once.
@@ -230,24 +220,11 @@ __device__ __forceinline__ void channel_drops(const Philox& gen, const GnDrop& d
 }
 
 template <typename T, int V, int ACT>
-__global__ __launch_bounds__(256) void gn_apply_kernel(const T* __restrict__ x, T* __restrict__ y, GnShape g, int gs,
-                                                       const double* __restrict__ part, const float* __restrict__ w,
-                                                       const float* __restrict__ b, float eps, GnDrop dr,
-                                                       double* __restrict__ stats) {
-    __shared__ double ms[2 * 64 * V];
+__global__ __launch_bounds__(256) void gn_apply_kernel(const T* __restrict__ x, T* __restrict__ y, GnShape g,
+                                                       const float* __restrict__ w, const float* __restrict__ b, GnDrop dr,
+                                                       const double* __restrict__ stats) {
     const GnPlace at(g);
-    const int slabw = g.tx * V;
-    group_stats(x, part, g, gs, at.img, at.slab, slabw, eps, ms);
-    const int first = at.slab * slabw, g0 = first / g.cpg;
-    if (at.chunk == 0 && stats) {  // for the backward pass; a group that spans slabs is written by the one it starts in
-        const int last = min(g.c, first + slabw);
-        for (int k = threadIdx.x; k <= (last - 1) / g.cpg - g0; k += 256)
-            if ((g0 + k) * g.cpg >= first) {
-                stats[((size_t)at.img * g.groups + g0 + k) * 2] = ms[2 * k];
-                stats[((size_t)at.img * g.groups + g0 + k) * 2 + 1] = ms[2 * k + 1];
-            }
-    }
-    const int c0 = first + ((int)threadIdx.x % g.tx) * V;
+    const int c0 = (at.slab * g.tx + (int)threadIdx.x % g.tx) * V;
     if (c0 >= g.c) return;
     const int ty = 256 / g.tx;
     Channel<ACT> ch[V];
@@ -255,13 +232,13 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const T* __restrict__ x, 
     const Philox gen(dr.rng);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int k = (c0 + e) / g.cpg - g0;
-        ch[e].set(ms[2 * k], ms[2 * k + 1], w ? w[c0 + e] : 1.f, b ? b[c0 + e] : 0.f);
+        const double* st = stats + ((size_t)at.img * g.groups + (c0 + e) / g.cpg) * 2;
+        ch[e].set(st[0], st[1], w ? w[c0 + e] : 1.f, b ? b[c0 + e] : 0.f);
     }
     channel_drops<V>(gen, dr, (unsigned long long)at.img * g.c + c0, ck);
     const size_t base = (size_t)at.img * g.hw * g.c + c0;
     const long long step = (long long)g.chunks * ty;
-    walk((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
+    walk<4>((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
         constexpr int N = decltype(nn)::value;
         float f[N][V];
 #pragma unroll
@@ -310,7 +287,7 @@ __global__ __launch_bounds__(256) void gn_bwd_stats_kernel(const T* __restrict__
         channel_drops<V>(gen, dr, (unsigned long long)at.img * g.c + c0, ck);
         const size_t base = (size_t)at.img * g.hw * g.c + c0;
         const long long step = (long long)g.chunks * ty;
-        walk((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
+        walk<2>((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
             constexpr int N = decltype(nn)::value;
             float f[N][V], d[N][V], sa[V], sq[V];
 #pragma unroll
@@ -441,7 +418,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const T* __restrict__
     channel_drops<V>(gen, dr, (unsigned long long)at.img * g.c + c0, ck);
     const size_t base = (size_t)at.img * g.hw * g.c + c0;
     const long long step = (long long)g.chunks * ty;
-    walk((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
+    walk<2>((long long)at.chunk * ty + threadIdx.x / g.tx, step, g.hw, [&](long long p, auto nn) {
         constexpr int N = decltype(nn)::value;
         float f[N][V], d[N][V];
 #pragma unroll
@@ -674,16 +651,14 @@ static bool gn_shape_ok(int n, long long hw, int c, int groups, int dtype) {
     return n > 0 && hw > 0 && c > 0 && groups > 0 && c % groups == 0 && vspw_dtype_ok(dtype) &&
            hw <= (0x7fffffffffffffffLL / n) / c / 8;
 }
-// 16-byte accesses when rows (for the group kernels: groups) keep the alignment; the plan is a function of the shape alone
-static int gn_vec(int c, int dtype) {
-    const int v = 16 / vspw_dtype_size(dtype);
-    return c % v == 0 ? v : 1;
-}
-#define GN_FWD_TRIPS 4
-#define GN_BWD_TRIPS 4
+// Four elements per access where rows (for the group kernels: groups) allow it.  (Eight 16-bit elements need twice the
+// registers per thread: [4,256,119,119] bf16 84 us in the four streaming kernels, four elements 69 us.)  The plan is a
+// function of the shape alone.
+static int gn_vec(int c) { return c % 4 == 0 ? 4 : 1; }
+#define GN_TRIPS 4
 #define GN_THREADS 256
-static GnShape gn_plan(int n, long long hw, int c, int groups, int dtype) {
-    const SlabPlan s = vspw_slab_plan(n, hw, c, gn_vec(c, dtype), 8, 2048);
+static GnShape gn_plan(int n, long long hw, int c, int groups) {
+    const SlabPlan s = vspw_slab_plan(n, hw, c, gn_vec(c), 8, 1024);
     GnShape g;
     g.hw = hw;
     g.n = n;
@@ -693,14 +668,11 @@ static GnShape gn_plan(int n, long long hw, int c, int groups, int dtype) {
     g.tx = s.tx;
     g.slabs = s.slabs;
     g.chunks = s.chunks;
-    g.trips = 0;
-    const int v = gn_vec(g.cpg, dtype);
+    const int v = gn_vec(g.cpg);
     g.fx = g.cpg / v;
-    if (g.fx <= GN_THREADS) {
-        const int ty = GN_THREADS / g.fx;
-        const long long t = (hw + ty - 1) / ty;
-        if (t <= GN_FWD_TRIPS && (long long)n * groups <= 0x7fffffffLL) g.trips = (int)t;
-    }
+    // Where it fits, one workgroup per image and group is one launch instead of three ([2,512,6,6]: 4.6 us against 12.6).  The
+    // same with 1024 threads for images up to 64 x 64 lost: [10,512,60,60] 61 us against 58 (320 workgroups on 256 CUs).
+    g.group = g.fx <= GN_THREADS && hw <= (long long)GN_TRIPS * (GN_THREADS / g.fx) && (long long)n * groups <= 0x7fffffffLL;
     return g;
 }
 static int gn_gs(const GnShape& g, int v) {  // groups that a slab can overlap
@@ -711,15 +683,15 @@ static int gn_gs(const GnShape& g, int v) {  // groups that a slab can overlap
 
 extern "C" size_t vspw_group_norm_fwd_workspace(int n, long long hw, int c, int groups, int dtype) {
     if (!gn_shape_ok(n, hw, c, groups, dtype)) return 0;
-    const GnShape g = gn_plan(n, hw, c, groups, dtype);
-    if (g.trips) return 0;
-    return (size_t)n * g.chunks * g.slabs * gn_gs(g, gn_vec(c, dtype)) * 2 * sizeof(double);
+    const GnShape g = gn_plan(n, hw, c, groups);
+    if (g.group) return 0;
+    return ((size_t)n * g.chunks * g.slabs * gn_gs(g, gn_vec(c)) + (size_t)n * groups) * 2 * sizeof(double);
 }
 
 extern "C" size_t vspw_group_norm_bwd_workspace(int n, long long hw, int c, int groups, int dtype) {
     if (!gn_shape_ok(n, hw, c, groups, dtype)) return 0;
-    const GnShape g = gn_plan(n, hw, c, groups, dtype);
-    return (size_t)n * ((g.trips ? 0 : g.chunks) + 1) * 2 * c * sizeof(double);
+    const GnShape g = gn_plan(n, hw, c, groups);
+    return (size_t)n * ((g.group ? 0 : g.chunks) + 1) * 2 * c * sizeof(double);
 }
 
 struct GnCall {
@@ -747,16 +719,21 @@ static int gn_fwd_launch(const GnCall& a) {
     const int gs = gn_gs(a.g, V);
     const dim3 grid((unsigned)(a.g.slabs * a.g.chunks * a.g.n));
     hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(256), 0, a.st, (const T*)a.x, a.g, gs, a.ws);
-    const int rc = vspw_launch_status();
+    int rc = vspw_launch_status();
     if (rc != VSPW_OK) return rc;
-    hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT>), grid, dim3(256), 0, a.st, (const T*)a.x, (T*)a.out, a.g, gs, a.ws, a.w, a.b,
-                       a.eps, a.dr, a.stats);
+    double* stats = a.stats ? a.stats : a.ws + (size_t)a.g.n * a.g.chunks * a.g.slabs * gs * 2;
+    const long long groups = (long long)a.g.n * a.g.groups;
+    hipLaunchKernelGGL((gn_finish_kernel<T>), dim3((unsigned)((groups + 3) / 4)), dim3(256), 0, a.st, (const T*)a.x, a.ws, a.g, gs,
+                       a.g.tx * V, a.eps, stats);
+    rc = vspw_launch_status();
+    if (rc != VSPW_OK) return rc;
+    hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT>), grid, dim3(256), 0, a.st, (const T*)a.x, (T*)a.out, a.g, a.w, a.b, a.dr, stats);
     return vspw_launch_status();
 }
 template <typename T, int V, int ACT>
 static int gn_fwd_group_launch(const GnCall& a) {
-    hipLaunchKernelGGL((gn_group_kernel<T, V, ACT, GN_FWD_TRIPS, GN_THREADS>), dim3((unsigned)(a.g.n * a.g.groups)), dim3(GN_THREADS),
-                       0, a.st, (const T*)a.x, (T*)a.out, a.g, a.w, a.b, a.eps, a.dr, a.stats);
+    hipLaunchKernelGGL((gn_group_kernel<T, V, ACT, GN_TRIPS, GN_THREADS>), dim3((unsigned)(a.g.n * a.g.groups)), dim3(GN_THREADS), 0,
+                       a.st, (const T*)a.x, (T*)a.out, a.g, a.w, a.b, a.eps, a.dr, a.stats);
     return vspw_launch_status();
 }
 
@@ -778,7 +755,7 @@ static int gn_bwd_launch(const GnCall& a) {
 }
 template <typename T, int V, int ACT>
 static int gn_bwd_group_launch(const GnCall& a) {
-    hipLaunchKernelGGL((gn_bwd_group_kernel<T, V, ACT, GN_BWD_TRIPS, GN_THREADS>), dim3((unsigned)(a.g.n * a.g.groups)),
+    hipLaunchKernelGGL((gn_bwd_group_kernel<T, V, ACT, GN_TRIPS, GN_THREADS>), dim3((unsigned)(a.g.n * a.g.groups)),
                        dim3(GN_THREADS), 0, a.st, (const T*)a.x, (const T*)a.dy, (T*)a.out, a.g, a.stats, a.w, a.b, a.dr, a.ws, a.dw,
                        a.db);
     const int rc = vspw_launch_status();
@@ -805,15 +782,14 @@ static int gn_act(const GnCall& a) {
 }
 template <typename T, bool BWD>
 static int gn_type(const GnCall& a, int v, int vg) {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (a.g.trips) return vg > 1 ? gn_act<T, V, true, BWD>(a) : gn_act<T, 1, true, BWD>(a);
-    return v > 1 ? gn_act<T, V, false, BWD>(a) : gn_act<T, 1, false, BWD>(a);
+    if (a.g.group) return vg > 1 ? gn_act<T, 4, true, BWD>(a) : gn_act<T, 1, true, BWD>(a);
+    return v > 1 ? gn_act<T, 4, false, BWD>(a) : gn_act<T, 1, false, BWD>(a);
 }
 template <bool BWD>
 static int gn_dispatch(const GnCall& a, int dtype) {
-    const int v = gn_vec(a.g.c, dtype), vg = gn_vec(a.g.cpg, dtype);
+    const int v = gn_vec(a.g.c), vg = gn_vec(a.g.cpg);
     if ((long long)a.g.slabs * a.g.chunks * a.g.n > 0x7fffffffLL || ((2LL * a.g.c + 31) / 32) * a.g.n > 0x7fffffffLL) return VSPW_EINVAL;
-    if (v > 1 && (((uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.out) & 15)) return VSPW_EINVAL;
+    if (v > 1 && (((uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.out) & 15)) return VSPW_EINVAL;  // storage on 16 bytes
     if (dtype == VSPW_F32) return gn_type<float, BWD>(a, v, vg);
     if (dtype == VSPW_BF16) return gn_type<bf16_t, BWD>(a, v, vg);
     return gn_type<f16_t, BWD>(a, v, vg);
@@ -825,7 +801,7 @@ extern "C" int vspw_group_norm_fwd(const void* x, void* y, int n, long long hw, 
     GnCall a = GnCall();
     if (!x || !y || !gn_shape_ok(n, hw, c, groups, dtype) || !(eps >= 0.f) || !gn_args(act, p, rng, channelwise, a.dr))
         return VSPW_EINVAL;
-    a.g = gn_plan(n, hw, c, groups, dtype);
+    a.g = gn_plan(n, hw, c, groups);
     const size_t need = vspw_group_norm_fwd_workspace(n, hw, c, groups, dtype);
     if (ws_bytes < need || (need && !ws)) return VSPW_EINVAL;
     a.x = x;
@@ -846,7 +822,7 @@ extern "C" int vspw_group_norm_bwd(const void* x, const void* dy, void* dx, int 
     GnCall a = GnCall();
     if (!x || !dy || !stats || !gn_shape_ok(n, hw, c, groups, dtype) || !gn_args(act, p, rng, channelwise, a.dr))
         return VSPW_EINVAL;
-    a.g = gn_plan(n, hw, c, groups, dtype);
+    a.g = gn_plan(n, hw, c, groups);
     if (!ws || ws_bytes < vspw_group_norm_bwd_workspace(n, hw, c, groups, dtype)) return VSPW_EINVAL;
     a.x = x;
     a.dy = dy;

@@ -634,7 +634,7 @@ int vspw_rng_next(long long* state, long long* used, void* stream);
 /* y = drop(act(w (x - mean) / sqrt(var + eps) + b)) on [n][hw][c] activations of type dtype, mean / var over the hw pixels and
  * the c / groups channels of a group; w, b (fp32 [c]) may be NULL; act 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf); p, rng,
  * channelwise as vspw_dropout (p = 0: none, rng may be NULL).  stats [n][groups][2] (fp64 mean and 1/sqrt(var + eps)) is
- * what the backward pass reads; NULL at inference.  16-byte aligned pointers where c is a multiple of 16 bytes. */
+ * what the backward pass reads; NULL at inference.  16-byte aligned pointers where c is a multiple of 4. */
 size_t vspw_group_norm_fwd_workspace(int n, long long hw, int c, int groups, int dtype);
 int vspw_group_norm_fwd(const void* x, void* y, int n, long long hw, int c, int groups, int dtype, const float* w,
                         const float* b, float eps, int act, double p, const long long* rng, int channelwise, double* stats,
