@@ -1,12 +1,14 @@
 """Differential attention (csrc/diff_attn.hip): softmax attention as the difference of two maps, fp32 and bf16, the maps never
 written.  The softmax counterpart of ops.non_local_dot for the non-local blocks."""
 import ctypes
+import functools
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _C
-from ._ops_norm import _DTYPES, _addr, _on_device, _raw_stream, _require_float, _same_device, _wants_grad
+from ._ops_norm import _DTYPES, _addr, _on_device, _raw_stream, _require_float, _require_ints, _same_device, _wants_grad
 from ._opbase import _Timed, _ktimer, _ws
 
 _ATTN_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -24,29 +26,65 @@ class AttnDesc(ctypes.Structure):
 _NEAR = 1 << 24  # strides between rows, maps and heads that the kernels address with 32 bits inside a tile (elements)
 
 
-def _strides(t):
-    """Element strides of all dimensions but the last, 0 where there is nothing to step over."""
-    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
-
-
-def _strided(t, g=1):
-    """(t, its strides) when the kernels can address it (dense last dimension, everything else on 16 bytes, near rows), else of
-    a copy.  g: how many heads a tile of rows mixes."""
-    st = _strides(t)
-    ve = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+def _strides(shape, stride, ve, g=1):
+    """The strides of all dimensions but the last, 0 where there is nothing to step over, and whether the kernels can address
+    them (dense last dimension, everything else on 16 bytes, near rows).  g: how many heads a tile of rows mixes."""
+    st = [0 if n == 1 else s for n, s in zip(shape[:-1], stride[:-1])]
+    ok = stride[-1] == 1
     for i, s in enumerate(st):
         ok = ok and s % ve == 0 and (i == 0 or (i == 2 and g == 1) or s * (g if i == 2 else 1) < _NEAR)
-    if not ok:
-        t = t.clone(memory_format=torch.contiguous_format)
-        st = _strides(t)
-    return t, st
+    return st, ok
 
 
-def _desc(q, k, lam, scale, frame, qs, ks, vs):
-    b, nq, h, _, d = q.shape
-    return AttnDesc(b, nq, k.shape[1], h, k.shape[2], d, _ATTN_DTYPES[q.dtype], _ATTN_DTYPES[lam.dtype], frame, scale,
-                    *qs, *ks, *vs)
+class _Plan:
+    __slots__ = ("desc", "ref", "fwd_bytes", "bwd_bytes", "q_ok", "k_ok", "v_ok", "empty", "frame", "scale")
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan(qd, kd, vd, ld, qs, ks, vs, ls, q_stride, k_stride, v_stride, scale, frame):
+    """Checks and descriptor of a call, a function of types, shapes and strides (a call for one token costs the host more than
+    the GPU)."""
+    if len(qs) != 5 or len(ks) != 5 or len(vs) != 4 or qs[3] != 2 or ks[3] != 2:
+        raise RuntimeError("diff_attention: q [B,Nq,H,2,D], k [B,Nk,Hk,2,D], v [B,Nk,Hk,2D] expected, got %s, %s, %s"
+                           % (tuple(qs), tuple(ks), tuple(vs)))
+    b, nq, h, _, d = qs
+    nk, hk = ks[1], ks[2]
+    _require_ints("diff_attention", b, nq, nk, h)
+    if ks[0] != b or ks[4] != d or tuple(vs) != (b, nk, hk, 2 * d):
+        raise RuntimeError("diff_attention: q %s, k %s and v %s do not belong together" % (tuple(qs), tuple(ks), tuple(vs)))
+    if h == 0 or hk == 0 or h % hk:
+        raise RuntimeError("diff_attention: %d query heads do not divide over %d key heads" % (h, hk))
+    if not diff_attention_supported(d):
+        raise RuntimeError("diff_attention: head width %d is not one of 16, 32, 64" % d)
+    if h * 2 * d >= _NEAR:
+        raise RuntimeError("diff_attention: %d heads of 2 x %d columns are more than a row may hold" % (h, d))
+    if kd != qd or vd != qd or ld not in (torch.float32, qd):
+        raise RuntimeError("diff_attention: q, k, v of one type and lam of that type or float32 expected, got %s, %s, %s, %s"
+                           % (qd, kd, vd, ld))
+    if tuple(ls) != (h,):
+        raise RuntimeError("diff_attention: lam must be [%d], got %s" % (h, tuple(ls)))
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    if not (0.0 < scale < float("inf")) or not ctypes.c_float(scale).value > 0.0:
+        raise ValueError("diff_attention: scale must be positive and finite, got %r" % scale)
+    if not 0 <= frame < 2 ** 31:
+        raise ValueError("diff_attention: frame must be a number of positions, got %r" % frame)
+    p = _Plan()
+    ve = 8 if qd == torch.bfloat16 else 4
+    qt, p.q_ok = _strides(qs, q_stride, ve, h // hk)
+    kt, p.k_ok = _strides(ks, k_stride, ve)
+    vt, p.v_ok = _strides(vs, v_stride, ve)
+    p.empty, p.frame, p.scale = 0 in (b, nq, nk), frame, scale
+    p.desc = AttnDesc(b, nq, nk, h, hk, d, _ATTN_DTYPES[qd], _ATTN_DTYPES[ld], frame, scale, *qt, *kt, *vt)
+    p.ref = ctypes.byref(p.desc)
+    p.fwd_bytes = 0 if p.empty else _C.query("vspw_diff_attn_fwd_workspace", p.ref)
+    p.bwd_bytes = 0 if p.empty else _C.query("vspw_diff_attn_bwd_workspace", p.ref)
+    return p
+
+
+def _plan_of(q, k, v, lam, scale, frame):
+    return _plan(q.dtype, k.dtype, v.dtype, lam.dtype, q.shape, k.shape, v.shape, lam.shape, q.stride(), k.stride(), v.stride(),
+                 scale, frame)
 
 
 def _flops(q, k, frame, per_pair):
@@ -57,45 +95,49 @@ def _flops(q, k, frame, per_pair):
     return per_pair * b * h * d * pairs
 
 
-def _timed(name, q, k, frame, per_pair):
+def _launch(name, q, k, frame, per_pair, *args):
     if not _ktimer["on"]:
-        return _Timed(name, 0.0)
-    return _Timed(name, _flops(q, k, frame, per_pair), "diff_attn b%d n%d/%d h%d d%d" % (q.shape[0], q.shape[1], k.shape[1],
-                                                                                          q.shape[2], q.shape[4]))
+        return _C.call("vspw_" + name, *args)
+    with _Timed(name, _flops(q, k, frame, per_pair), "diff_attn b%d n%d/%d h%d d%d" % (q.shape[0], q.shape[1], k.shape[1],
+                                                                                      q.shape[2], q.shape[4])):
+        _C.call("vspw_" + name, *args)
 
 
 @_on_device
-def _attn_fwd(q, k, v, lam, scale, mask, frame, train):
-    """(out, maps, lse, descriptor, q, k, v): the last three as the kernels read them"""
-    hk = k.shape[2]
+def _attn_fwd(q, k, v, lam, mask, plan, train):
+    """(out, maps, lse, plan, q, k, v): the last three as the kernels read them (a copy where they cannot address a tensor)"""
     b, nq, h, _, d = q.shape
-    (q, qs), (k, ks), (v, vs) = _strided(q, h // hk), _strided(k), _strided(v)
-    out = torch.empty((b, nq, h, 2 * d), device=q.device, dtype=q.dtype)
+    dev = q.device
+    out = torch.empty((b, nq, h, 2 * d), device=dev, dtype=q.dtype)
     maps = lse = None
-    if not out.numel() or not k.shape[1]:
-        return out.zero_(), None, None, None, q, k, v
+    if plan.empty:
+        return out.zero_(), None, None, plan, q, k, v
+    qa, ka, va = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not (plan.q_ok and plan.k_ok and plan.v_ok) or (qa | ka | va) % 16:
+        q = q if plan.q_ok and qa % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+        k = k if plan.k_ok and ka % 16 == 0 else k.clone(memory_format=torch.contiguous_format)
+        v = v if plan.v_ok and va % 16 == 0 else v.clone(memory_format=torch.contiguous_format)
+        plan = _plan_of(q, k, v, lam, plan.scale, plan.frame)
+        qa, ka, va = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if train:
-        maps = torch.empty((b, nq, h, 2, 2 * d), device=q.device, dtype=torch.float32)
-        lse = torch.empty((2, b * hk, nq * (h // hk)), device=q.device, dtype=torch.float32)
-    ds = _desc(q, k, lam, scale, frame, qs, ks, vs)
-    ref = ctypes.byref(ds)
-    nbytes = _C.query("vspw_diff_attn_fwd_workspace", ref)
-    ws = _ws(nbytes, q.device) if nbytes else None
-    with _timed("diff_attn_fwd", q, k, frame, 12.0):
-        _C.call("vspw_diff_attn_fwd", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(mask), out.data_ptr(),
-                _addr(maps), _addr(lse), _addr(ws), nbytes, _raw_stream(q.device.index))
-    return out, maps, lse, ds, q, k, v
+        maps = torch.empty((b, nq, h, 2, 2 * d), device=dev, dtype=torch.float32)
+        lse = torch.empty((2, b, h, nq), device=dev, dtype=torch.float32)
+    nbytes = plan.fwd_bytes
+    ws = _ws(nbytes, dev) if nbytes else None
+    _launch("diff_attn_fwd", q, k, plan.frame, 12.0, plan.ref, qa, ka, va, lam.data_ptr(), _addr(mask), out.data_ptr(), _addr(maps),
+            _addr(lse), _addr(ws), nbytes, _raw_stream(dev.index))
+    return out, maps, lse, plan, q, k, v
 
 
 @_on_device
-def _attn_bwd(q, k, v, lam, mask, maps, lse, ds, go, frame, need):
+def _attn_bwd(q, k, v, lam, mask, maps, lse, plan, go, need):
     dev, dt = q.device, q.dtype
     dq = torch.empty(q.shape, device=dev, dtype=dt) if need[0] else None
     dk = dv = None
     if need[1] or need[2]:
         dk, dv = torch.empty(k.shape, device=dev, dtype=dt), torch.empty(v.shape, device=dev, dtype=dt)
     dlam = torch.empty_like(lam) if need[3] else None
-    if maps is None:  # no rows or no keys
+    if plan.empty:
         for t in (dq, dk, dv, dlam):
             if t is not None:
                 t.zero_()
@@ -103,13 +145,11 @@ def _attn_bwd(q, k, v, lam, mask, maps, lse, ds, go, frame, need):
     go = go.contiguous()
     if go.data_ptr() % 16:
         go = go.clone()
-    ref = ctypes.byref(ds)
-    nbytes = _C.query("vspw_diff_attn_bwd_workspace", ref)
+    nbytes = plan.bwd_bytes
     ws = _ws(nbytes, dev)
-    with _timed("diff_attn_bwd", q, k, frame, 28.0):
-        _C.call("vspw_diff_attn_bwd", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(mask), maps.data_ptr(),
-                lse.data_ptr(), go.data_ptr(), _addr(dq), _addr(dk), _addr(dv), _addr(dlam), ws.data_ptr(), nbytes,
-                _raw_stream(dev.index))
+    _launch("diff_attn_bwd", q, k, plan.frame, 28.0, plan.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _addr(mask),
+            maps.data_ptr(), lse.data_ptr(), go.data_ptr(), _addr(dq), _addr(dk), _addr(dv), _addr(dlam), ws.data_ptr(), nbytes,
+            _raw_stream(dev.index))
     return dq, dk, dv, dlam
 
 
@@ -117,19 +157,18 @@ class DiffAttentionFn(torch.autograd.Function):
     """Forward keeps both maps' outputs in float32 and their log-sum-exps; backward recomputes the scores."""
 
     @staticmethod
-    def forward(ctx, q, k, v, lam, scale, mask, frame):
-        out, maps, lse, ds, q, k, v = _attn_fwd(q, k, v, lam, scale, mask, frame, True)
-        ctx.meta = (ds, frame)
+    def forward(ctx, q, k, v, lam, mask, plan):
+        out, maps, lse, ctx.plan, q, k, v = _attn_fwd(q, k, v, lam, mask, plan, True)
         ctx.save_for_backward(q, k, v, lam, mask, maps, lse)
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, go):
         q, k, v, lam, mask, maps, lse = ctx.saved_tensors
-        ds, frame = ctx.meta
         need = ctx.needs_input_grad
-        dq, dk, dv, dlam = _attn_bwd(q, k, v, lam, mask, maps, lse, ds, go, frame, need)
-        return dq, dk if need[1] else None, dv if need[2] else None, dlam, None, None, None
+        dq, dk, dv, dlam = _attn_bwd(q, k, v, lam, mask, maps, lse, ctx.plan, go, need)
+        return dq, dk if need[1] else None, dv if need[2] else None, dlam, None, None
 
 
 def diff_attention_supported(d):
@@ -145,44 +184,22 @@ def diff_attention(q, k, v, lam, scale=None, key_mask=None, frame=0):
     lam [H]: float32 or the inputs' type.  scale: default 1 / sqrt(D), must be positive.  key_mask [B,Nk] bool: True where the
     key takes part; what masked positions hold (infinities, NaN) is not used.  frame > 0: positions come in frames of that
     many, and a query sees the keys of its own frame and of earlier ones, the ends of queries and keys aligned (query i stands
-    at position i + Nk - Nq).  A query without keys gets zeros and zero gradients.
+    at position i + Nk - Nq); keys and values that frame hides from some queries must be finite.  A query without keys gets
+    zeros and zero gradients.
     """
-    _require_float(q, "diff_attention", _ATTN_DTYPES)
-    for t in (k, v, lam):
+    for t in (q, k, v, lam):
         _require_float(t, "diff_attention", _ATTN_DTYPES)
     _same_device("diff_attention", q, k, v, lam, key_mask)
-    if q.dim() != 5 or k.dim() != 5 or v.dim() != 4 or q.shape[3] != 2 or k.shape[3] != 2:
-        raise RuntimeError("diff_attention: q [B,Nq,H,2,D], k [B,Nk,Hk,2,D], v [B,Nk,Hk,2D] expected, got %s, %s, %s"
-                           % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    b, nq, h, _, d = q.shape
-    nk, hk = k.shape[1], k.shape[2]
-    if k.shape[0] != b or k.shape[4] != d or tuple(v.shape) != (b, nk, hk, 2 * d):
-        raise RuntimeError("diff_attention: q %s, k %s and v %s do not belong together"
-                           % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if h == 0 or hk == 0 or h % hk:
-        raise RuntimeError("diff_attention: %d query heads do not divide over %d key heads" % (h, hk))
-    if not diff_attention_supported(d):
-        raise RuntimeError("diff_attention: head width %d is not one of 16, 32, 64" % d)
-    if k.dtype != q.dtype or v.dtype != q.dtype or lam.dtype not in (torch.float32, q.dtype):
-        raise RuntimeError("diff_attention: q, k, v of one type and lam of that type or float32 expected, got %s, %s, %s, %s"
-                           % (q.dtype, k.dtype, v.dtype, lam.dtype))
-    if tuple(lam.shape) != (h,):
-        raise RuntimeError("diff_attention: lam must be [%d], got %s" % (h, tuple(lam.shape)))
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not (0.0 < scale < float("inf")) or not ctypes.c_float(scale).value > 0.0:
-        raise ValueError("diff_attention: scale must be positive and finite, got %r" % scale)
-    frame = int(frame)
-    if not 0 <= frame < 2 ** 31:
-        raise ValueError("diff_attention: frame must be a number of positions, got %r" % frame)
+    plan = _plan_of(q, k, v, lam, None if scale is None else float(scale), int(frame))
     if key_mask is not None:
-        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (b, nk):
-            raise RuntimeError("diff_attention: key_mask must be bool [%d,%d], got %s %s"
-                               % (b, nk, key_mask.dtype, tuple(key_mask.shape)))
+        if key_mask.dtype != torch.bool or key_mask.shape != k.shape[:2]:
+            raise RuntimeError("diff_attention: key_mask must be bool %s, got %s %s"
+                               % (list(k.shape[:2]), key_mask.dtype, tuple(key_mask.shape)))
         key_mask = key_mask.contiguous()
     lam = lam.contiguous()
     if _wants_grad(q, k, v, lam):
-        return DiffAttentionFn.apply(q, k, v, lam, scale, key_mask, frame)
-    return _attn_fwd(q, k, v, lam, scale, key_mask, frame, False)[0]
+        return DiffAttentionFn.apply(q, k, v, lam, key_mask, plan)
+    return _attn_fwd(q, k, v, lam, key_mask, plan, False)[0]
 
 
 @_on_device
@@ -211,6 +228,7 @@ class DiffLambdaFn(torch.autograd.Function):
         return _lambda_fwd(lq1, lk1, lq2, lk2, init)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         return _lambda_bwd(*ctx.saved_tensors, g) + (None,)
 

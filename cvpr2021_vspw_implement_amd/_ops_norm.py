@@ -5,8 +5,10 @@ Both work on channels-last memory like the rest of ops.py: a [N,C,...] tensor is
 when it is already there) and the result comes back in that order under the input's logical shape.
 """
 import functools
+import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _C
 from ._opbase import _ws, to_nhwc
@@ -30,6 +32,11 @@ def _require_float(t, what, dtypes=_DTYPES):
                            "there is no CPU fallback" % (what, t.device))
     if t.dtype not in dtypes:
         raise RuntimeError("%s: %s tensors only (got %s)" % (what, " / ".join(str(d)[6:] for d in dtypes), t.dtype))
+
+
+def _require_ints(what, *sizes):
+    if max(sizes) >= 2 ** 31:
+        raise RuntimeError("%s: sizes below 2^31 only, got %s" % (what, sizes))
 
 
 def _same_device(what, first, *others):
@@ -63,7 +70,7 @@ def _wants_grad(*ts):
 
 def _rows(x):
     """[N,C,...] of any strides -> ([N][pixels][C] memory under the logical shape [N,C,P,1], its 4-D tensor)."""
-    x4 = x if x.dim() == 4 else x.reshape(x.shape[0], x.shape[1], -1, 1)
+    x4 = x if x.dim() == 4 else x.reshape(x.shape[0], x.shape[1], math.prod(x.shape[2:]), 1)
     if x4.is_contiguous(memory_format=torch.channels_last):
         return x4
     if x4.dtype == torch.float32 and x4.is_contiguous() and x4.numel():
@@ -114,6 +121,7 @@ class DropoutFn(torch.autograd.Function):
         return _dropout(x, p, rng, channelwise)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         return _dropout(g, ctx.meta[0], ctx.saved_tensors[0], ctx.meta[1]), None, None, None
 
@@ -132,6 +140,8 @@ def dropout(x, p, rng=None, channelwise=False):
     _same_device("dropout", x, rng)
     if channelwise and x.dim() < 2:
         raise RuntimeError("dropout: channelwise needs a [N,C,...] tensor, got %s" % (tuple(x.shape),))
+    if channelwise or x.dim() > 2:
+        _require_ints("dropout", x.shape[0], x.shape[1])
     if _wants_grad(x):
         return DropoutFn.apply(x, p, rng, bool(channelwise))
     return _dropout(x, p, rng, channelwise)
@@ -149,7 +159,9 @@ def rng_next(state):
     advances by one - on the stream, so every replay of a captured step draws a new mask."""
     if not state.is_cuda or state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous():
         raise RuntimeError("rng_next: two contiguous int64 values (seed, offset) on the GPU expected")
-    return _rng_next(state)
+    used = _rng_next(state)
+    torch.autograd.graph.increment_version(state)  # written outside autograd's sight: a graph that saved it has to notice
+    return used
 
 
 # --------------------------------------------------------------------------------------------------------- group norm
@@ -213,6 +225,7 @@ class GroupNormActFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         xr, weight, bias, rng, stats = ctx.saved_tensors
         return _norm_bwd(xr, g, weight, bias, rng, stats, ctx.meta, ctx.needs_input_grad) + (None, None)
@@ -226,6 +239,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     if x.dim() < 2:
         raise RuntimeError("group_norm_act: a [N,C,...] tensor expected, got %s" % (tuple(x.shape),))
     c = x.shape[1]
+    _require_ints("group_norm_act", x.shape[0], c)
     num_groups = int(num_groups)
     if num_groups <= 0 or c % num_groups or c == 0:
         raise ValueError("group_norm_act: %d channels do not divide into %d groups" % (c, num_groups))

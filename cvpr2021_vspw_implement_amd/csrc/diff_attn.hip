@@ -1272,6 +1272,8 @@ static int da_parts(long long nb, int nt, int slots, int extra, int most) {
 }
 static int da_span(int n, int parts) { return vspw_cdiv(vspw_cdiv(n, DA_TILE), parts) * DA_TILE; }
 
+#define DA_NEAR (1LL << 24)  // elements: 64 rows of a tile times 4 bytes stay below 2^32
+
 struct DaPlan {
     int g, rows, wn, tiles, parts, span;              // forward
     int qt, qparts, qspan, kt, kparts, kspan, lchunks;  // backward
@@ -1291,6 +1293,7 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
         return false;
     p.rows = (int)rows;
     const int W = 2 * d->d, nt = vspw_cdiv(d->nk, DA_TILE);
+    if ((long long)d->h * W >= DA_NEAR) return false;  // a row of the output and of its gradient
     // up to 32 rows: single-wave workgroups, many parts of the key axis; else four waves share a key tile
     p.wn = p.rows <= 32 ? 1 : 4;
     p.tiles = vspw_cdiv(p.rows, 32 * p.wn);
@@ -1323,8 +1326,6 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     p.bwd_bytes += 32;  // alignment of the pieces
     return true;
 }
-#define DA_NEAR (1LL << 24)  // elements: 32 rows of a tile times 4 bytes stay below 2^31
-
 static bool da_strides_ok(const vspw_dattn_desc* d, const DaPlan& p, const void* q, const void* k, const void* v) {
     const long long ve = d->dtype == VSPW_F32 ? 4 : 8;
     const long long s[] = {d->q_sb, d->q_sn, d->q_sh, d->q_sm, d->k_sb, d->k_sn, d->k_sh, d->k_sm, d->v_sb, d->v_sn, d->v_sh};

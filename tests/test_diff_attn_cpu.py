@@ -86,3 +86,15 @@ def test_workspaces_hold_whole_parts():
         n = _C.query("vspw_diff_attn_fwd_workspace", ctypes.byref(desc(b=b, nq=nq, nk=nk, h=h, hk=hk, d=d)))
         row = b * h * nq * (4 * d + 4) * 4
         assert n % row == 0 and n // row != 1 and n // row <= (nk + 31) // 32
+
+
+def test_rows_that_outgrow_the_offsets_are_refused():
+    """Offsets inside a tile of 64 rows are 32 bits wide: the heads of a position, and each near stride, stay below 2^24."""
+    from cvpr2021_vspw_implement_amd import _C
+
+    def nbytes(**kw):
+        return _C.query("vspw_diff_attn_bwd_workspace", ctypes.byref(desc(**kw)))
+
+    assert nbytes(h=1 << 17, hk=1, d=32, nq=2, nk=2) > 0
+    assert nbytes(h=1 << 18, hk=1 << 18, d=32, nq=2, nk=2) == 0
+    assert nbytes(h=1 << 17, hk=1 << 17, d=64, nq=2, nk=2) == 0

@@ -343,3 +343,31 @@ def test_refusals(dev):
             ops.diff_attention(q, k, v, lam, **kw)
     with pytest.raises(RuntimeError):
         ops.diff_lambda(lam, lam, lam, lam, 0.1)
+
+
+def test_a_second_derivative_is_refused(dev):
+    from cvpr2021_vspw_implement_amd import ops
+
+    ts = [t.to(dev).requires_grad_(True) for t in inputs(1, 4, 6, 2, 1, 16, "f32")[:4]]
+    out = ops.diff_attention(*ts)
+    g, = torch.autograd.grad((out * out).sum(), ts[0], create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_many_layouts_of_one_shape(dev):
+    """Calls whose types and shapes agree and whose strides, alignment and scale differ."""
+    from cvpr2021_vspw_implement_amd import ops
+
+    q, k, v, lam, go = (t.to(dev) for t in inputs(2, 70, 70, 4, 2, 16, "f32"))
+    big = torch.zeros(q.numel() + 4, device=dev)
+    odd = big[1:1 + q.numel()].view(q.shape).copy_(q)  # 4 bytes past a boundary
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)
+    for scale in (None, 0.5):
+        a = ops.diff_attention(q, k, v, lam, scale)
+        for other in (odd, turned, q.clone()):
+            leaf = other.detach().requires_grad_(True)
+            b = ops.diff_attention(leaf, k, v, lam, scale)
+            g, = torch.autograd.grad(b, leaf, go)
+            assert torch.equal(a, b) and g.shape == q.shape
+    assert not torch.equal(ops.diff_attention(q, k, v, lam, 0.5), ops.diff_attention(q, k, v, lam, 0.25))

@@ -401,3 +401,38 @@ def test_fused_sequential_equals_the_separate_calls(dev):
     y = bn(x)
     k = keep64((2, 32, 7, 6), 0.2, torch.tensor([5, 0]), True)
     assert ((y.cpu() != 0) <= (k != 0)).all() and (y != 0).any()
+
+
+def test_a_second_derivative_is_refused(dev):
+    from cvpr2021_vspw_implement_amd import ops
+
+    x = torch.randn(2, 8, 4, 4, device=dev, requires_grad=True)
+    for y in (ops.group_norm_act(x, 4), ops.dropout(x, 0.5, make_rng(dev, 1))):
+        g, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
+def test_a_state_that_moved_on_is_noticed(dev):
+    """The backward pass recomputes the mask: a state that advanced since the forward pass is an error, not another mask."""
+    from cvpr2021_vspw_implement_amd import ops
+
+    state = make_rng(dev, 5)
+    x = torch.randn(2, 8, 4, 4, device=dev, requires_grad=True)
+    for y in (ops.dropout(x, 0.5, state), ops.group_norm_act(x, 4, p=0.5, rng=state)):
+        ops.rng_next(state)
+        with pytest.raises(RuntimeError):
+            y.sum().backward()
+
+
+@pytest.mark.parametrize("shape", [(0, 8, 5), (0, 8), (2, 8, 0), (0, 8, 3, 3), (2, 8, 2, 0, 3)])
+def test_empty(dev, shape):
+    from cvpr2021_vspw_implement_amd import ops
+
+    w = torch.ones(8, device=dev, requires_grad=True)
+    x = torch.randn(shape, device=dev, requires_grad=True)
+    for channelwise in (False, True):
+        y = ops.dropout(ops.group_norm_act(x, 4, w), 0.5, make_rng(dev, 1), channelwise)
+        assert y.shape == shape
+        gx, gw = torch.autograd.grad(y.sum(), (x, w))
+        assert gx.shape == shape and (gw == 0).all()
