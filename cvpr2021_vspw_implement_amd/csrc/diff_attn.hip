@@ -190,6 +190,38 @@ __device__ __forceinline__ int da_limit(const DaArgs& a, int row) {
     const long long lim = (pos / a.frame + 1) * a.frame;
     return lim < a.nk ? (int)lim : a.nk;
 }
+// The first row (a multiple of DA_TILE) that sees keys from `key` on, which may lie behind the last one.
+__device__ __forceinline__ long long da_first_row(const DaArgs& a, int key) {
+    const long long q0 = (long long)(key / a.frame) * a.frame - a.nk + a.nq;
+    return q0 > 0 ? q0 * a.g / DA_TILE * DA_TILE : 0;
+}
+// With frames the parts that stream nothing write nothing, and a tile with a single part left writes its result itself.
+// Parts [0, n) of the rows' tile that ends with row `last`, and [n, parts) of the keys' tile that begins with `key`:
+__device__ __forceinline__ int da_row_parts(const DaArgs& a, int last) {
+    return a.frame ? max(0, da_limit(a, last) - 1) / a.span + 1 : a.parts;
+}
+__device__ __forceinline__ int da_key_parts(const DaArgs& a, int key) {
+    return a.frame ? (int)min(da_first_row(a, key) / a.span, (long long)a.parts - 1) : 0;
+}
+// The workgroup's place.  With frames the parts that every tile has come first, and among them the longest tiles (rows: the
+// last, keys: the first); neighbours, which go to different XCDs, then have like lengths.
+__device__ __forceinline__ void da_place(const DaArgs& a, bool keys, int& tile, int& part, int& bh) {
+    const int x = blockIdx.x;
+    if (a.frame) {
+        const int nb = a.b * a.hk;
+        bh = x % nb;
+        tile = x / nb % a.tiles;
+        part = x / nb / a.tiles;
+        if (keys)
+            part = a.parts - 1 - part;
+        else
+            tile = a.tiles - 1 - tile;
+    } else {
+        tile = x % a.tiles;
+        part = x / a.tiles % a.parts;
+        bh = x / a.tiles / a.parts;
+    }
+}
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
@@ -323,11 +355,10 @@ struct RowOf {
     int bi, kh, part, block0, row0, row, head, qi;
     bool live;
     __device__ __forceinline__ RowOf(const DaArgs& a, int wn, int wave, int l31) {
-        const int tile = blockIdx.x % a.tiles;
-        const int rest = blockIdx.x / a.tiles;
-        part = rest % a.parts;
-        bi = rest / a.parts / a.hk;
-        kh = rest / a.parts % a.hk;
+        int tile, bh;
+        da_place(a, false, tile, part, bh);
+        bi = bh / a.hk;
+        kh = bh % a.hk;
         block0 = tile * 32 * wn;
         row0 = block0 + wave * 32;
         live = row0 + l31 < a.rows;
@@ -356,6 +387,8 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lh = lane >> 5;
     const RowOf ro(a, WN, wave, l31);
+    const int nparts = da_row_parts(a, ro.last(a, WN));
+    if (ro.part >= nparts) return;
     const T* qrow = reinterpret_cast<const T*>(a.q) + ro.bi * a.q_sb + ro.qi * a.q_sn + ro.head * a.q_sh;
     Frag q1[KC], q2[KC];
 #pragma unroll
@@ -553,7 +586,7 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
     l2 += __shfl_xor(l2, 32, 64);
     if (!ro.live) return;
     const size_t e = ((size_t)ro.bi * a.hk + ro.kh) * a.rows + ro.row, n = (size_t)a.b * a.hk * a.rows;
-    if (a.parts > 1) {  // unnormalised sums with their maximum, joined by da_join_kernel
+    if (nparts > 1) {  // unnormalised sums with their maximum, joined by da_join_kernel
         float* po = a.part + (ro.part * n + e) * 2 * W;
 #pragma unroll
         for (int j = 0; j < CB; ++j)
@@ -589,6 +622,10 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
 
 // Joins the parts of a row.  Up to 32 parts: W / 4 threads per row, each goes over the parts by itself (every thread of a row
 // reads the same maxima and sums of weights, from the cache).
+__device__ __forceinline__ int da_last_of(const DaArgs& a, int row) {  // the last row of the forward kernel's tile
+    const int n = a.rows <= 32 ? 32 : 128;
+    return min(row / n * n + n, a.rows) - 1;
+}
 template <typename T, int D>
 __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
     constexpr int W = 2 * D, CT = W / 4;
@@ -597,8 +634,10 @@ __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
     const int ch = 4 * (threadIdx.x % CT);
     const int bh = (int)(e / a.rows), row = (int)(e % a.rows);
     const int head = (bh % a.hk) * a.g + row % a.g;
+    const int nparts = da_row_parts(a, da_last_of(a, row));
+    if (nparts == 1) return;
     float M1 = -DA_INF, M2 = -DA_INF, L1 = 0.f, L2 = 0.f;
-    for (int p = 0; p < a.parts; ++p) {
+    for (int p = 0; p < nparts; ++p) {
         const f32x4 v = *reinterpret_cast<const f32x4*>(a.ml + (p * n + e) * 4);
         M1 = fmaxf(M1, v[0]);
         M2 = fmaxf(M2, v[2]);
@@ -606,7 +645,7 @@ __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
     const float u1 = M1 == -DA_INF ? 0.f : M1, u2 = M2 == -DA_INF ? 0.f : M2;
     f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
 #pragma unroll 4
-    for (int p = 0; p < a.parts; ++p) {
+    for (int p = 0; p < nparts; ++p) {
         const f32x4 v = *reinterpret_cast<const f32x4*>(a.ml + (p * n + e) * 4);
         const float* s = a.part + (p * n + e) * 2 * W + ch;
         const float w1 = exp2f(v[0] - u1), w2 = exp2f(v[2] - u2);
@@ -639,8 +678,10 @@ __global__ __launch_bounds__(256) void da_join_row_kernel(const DaArgs a) {
     const size_t n = (size_t)a.b * a.hk * a.rows, e = blockIdx.x;
     const int bh = (int)(e / a.rows), row = (int)(e % a.rows);
     const int head = (bh % a.hk) * a.g + row % a.g;
+    const int nparts = da_row_parts(a, da_last_of(a, row));
+    if (nparts == 1) return;
     const f32x4 none = {-DA_INF, 0.f, -DA_INF, 0.f};
-    const f32x4 mine = tid < a.parts ? *reinterpret_cast<const f32x4*>(a.ml + (tid * n + e) * 4) : none;  // at most 256 parts
+    const f32x4 mine = tid < nparts ? *reinterpret_cast<const f32x4*>(a.ml + (tid * n + e) * 4) : none;  // at most 256 parts
     float u[2], L[2];
     const float w1 = wave_max(mine[0]), w2 = wave_max(mine[2]);
     if ((tid & 63) == 0) {
@@ -661,7 +702,7 @@ __global__ __launch_bounds__(256) void da_join_row_kernel(const DaArgs a) {
     const int ch = tid % CT, map = ch >= CT / 2 ? 1 : 0;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int p = tid / CT; p < a.parts; p += PT)
+    for (int p = tid / CT; p < nparts; p += PT)
         acc += *reinterpret_cast<const f32x4*>(a.part + (p * n + e) * 2 * W + 4 * ch) * exp2f(a.ml[(p * n + e) * 4 + 2 * map] - u[map]);
     sum[tid] = acc;
     __syncthreads();
@@ -766,6 +807,8 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lh = lane >> 5;
     const RowOf ro(a, 4, wave, l31);
+    const int nparts = da_row_parts(a, ro.last(a, 4));
+    if (ro.part >= nparts) return;
     const size_t n = (size_t)a.b * a.hk * a.rows, e0 = ((size_t)ro.bi * a.hk + ro.kh) * a.rows + ro.row;
     const size_t o = (((size_t)ro.bi * a.nq + ro.qi) * a.h + ro.head) * W;
     const T* qrow = reinterpret_cast<const T*>(a.q) + ro.bi * a.q_sb + ro.qi * a.q_sn + ro.head * a.q_sh;
@@ -941,7 +984,7 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
             const f32x4 x = quad(g1[j], g4) * a.scale, y = quad(g2[j], g4) * f2;
             // D = 16: map 1 sits in channels 0..15 of its product, map 2 in channels 16..31 of its own
             const bool ok1 = D >= 32 || ch < D, ok2 = D >= 32 || ch >= D;
-            if (a.parts > 1) {
+            if (nparts > 1) {
                 float* p = a.part + (size_t)ro.part * a.b * a.nq * a.h * W + o;
                 if (ok1) *reinterpret_cast<f32x4*>(p + ch) = x;
                 if (ok2) *reinterpret_cast<f32x4*>(p + C2 + ch) = y;
@@ -966,11 +1009,12 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     __shared__ __attribute__((aligned(16))) float Rs[4][6][DA_TILE];  // lse 1, lse 2, D_1, D_2, lambda, key limit (int)
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lh = lane >> 5;
-    const int tile = blockIdx.x % a.tiles;
-    const int rest = blockIdx.x / a.tiles;
-    const int part = rest % a.parts, bh = rest / a.parts;
+    int tile, part, bh;
+    da_place(a, true, tile, part, bh);
     const int bi = bh / a.hk, kh = bh % a.hk;
     const int block0 = tile * 128;
+    const int part0 = da_key_parts(a, block0);
+    if (part < part0) return;
     const int key = block0 + wave * 32 + l31;
     const bool live = key < a.nk && (!a.mask || a.mask[(size_t)bi * a.nk + min(key, a.nk - 1)]);
     const size_t n = (size_t)a.b * a.hk * a.rows;
@@ -992,9 +1036,9 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     const int row_end = min(a.rows, row_begin + a.span);
     int nedge = 0;   // leading tiles with rows that do not see all of the workgroup's keys (rows see more and more of them)
     if (a.frame) {
-        const long long shift = a.nk - a.nq, first = block0, last = min(block0 + 128, a.nk) - 1;
-        const long long q0 = first / a.frame * a.frame - shift, q1 = last / a.frame * a.frame - shift;
-        const long long r0 = q0 > 0 ? q0 * a.g / DA_TILE * DA_TILE : 0;  // the first row that sees the first key
+        const int last = min(block0 + 128, a.nk) - 1;
+        const long long q1 = (long long)(last / a.frame) * a.frame - a.nk + a.nq;
+        const long long r0 = da_first_row(a, block0);  // the first row that sees the first key
         if (r0 > row_begin) row_begin = r0 < row_end ? (int)r0 : row_end;
         const long long r1 = q1 * a.g - row_begin;  // the first row that sees the last key
         nedge = r1 > 0 ? (int)min((r1 + DA_TILE - 1) / DA_TILE, (long long)INT_MAX) : 0;
@@ -1197,7 +1241,7 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     const size_t all = (size_t)a.b * a.nk * a.hk * W;
     auto out = [&](int which, int ch, f32x4 x) {
         if (!live) x = f32x4{0.f, 0.f, 0.f, 0.f};  // whatever a hidden key's column holds, it never left this lane
-        if (a.parts > 1)
+        if (part0 + 1 < a.parts)
             *reinterpret_cast<f32x4*>(a.part + ((size_t)part * 2 + which) * all + o + ch) = x;
         else
             M::store4(reinterpret_cast<T*>(which == 0 ? a.dk : a.dv) + o + ch, x);
@@ -1216,13 +1260,25 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     }
 }
 
-// out = sum over parts of part[p * stride + i], rounded once
-template <typename T>
-__global__ __launch_bounds__(256) void da_sum_kernel(const float* __restrict__ part, T* __restrict__ out, long long n4,
-                                                     int parts, long long stride) {
+// out = sum over the parts that were written, part[p * stride + i], rounded once.  KEYS: dk or dv [b][nk][hk][w], else dq
+// [b][nq][h][w].
+template <typename T, bool KEYS>
+__global__ __launch_bounds__(256) void da_sum_kernel(const DaArgs a, const float* __restrict__ part, T* __restrict__ out,
+                                                     long long n4, long long stride, int w4) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
-        f32x4 s = *reinterpret_cast<const f32x4*>(part + 4 * i);
-        for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(part + p * stride + 4 * i);
+        int p0 = 0, p1 = a.parts;
+        if (a.frame) {
+            const long long x = i / w4;
+            if (KEYS) {
+                p0 = da_key_parts(a, (int)(x / a.hk % a.nk) / 128 * 128);
+            } else {
+                const int row = (int)(x / a.h % a.nq) * a.g + (int)(x % a.h) % a.g;
+                p1 = da_row_parts(a, min(row / 128 * 128 + 128, a.rows) - 1);
+            }
+            if (p0 + 1 >= p1) continue;
+        }
+        f32x4 s = *reinterpret_cast<const f32x4*>(part + p0 * stride + 4 * i);
+        for (int p = p0 + 1; p < p1; ++p) s += *reinterpret_cast<const f32x4*>(part + p * stride + 4 * i);
         Mx<T>::store4(out + 4 * i, s);
     }
 }
@@ -1270,6 +1326,67 @@ static int da_parts(long long nb, int nt, int slots, int extra, int most) {
     }
     return best;
 }
+// The same with frames, where the tiles of rows or keys stream different lengths (up to 8 of them are looked at) and the
+// longest begin first: the end of that schedule, and `join` tiles for reading a piece again.  bf16, 2 x 4 frames of 961, 4 heads
+// on 2 of 64: forward 192 us in one part, 163 + 13 in two, 152 + 19 in three (taken), 171 + 27 in five; dk and dv 263 us in two
+// (as without frames), 202 + 12 in three.
+#define DA_LENGTHS 8
+static int da_parts_frames(const int* len, int n, double each, int nt, int slots, int extra, double join, int most) {
+    int best = 1, span = 0;
+    double cost = 1e300;
+    const double rounds = 4.0 * slots / (n * each) + 4.0;  // more pieces than that no longer even anything out
+    if (rounds < most) most = (int)rounds;
+    for (int p = 1; p <= most && p <= nt; ++p) {
+        if (vspw_cdiv(nt, p) == span) continue;
+        span = vspw_cdiv(nt, p);
+        double at[DA_LENGTHS * 2 + 2], count[DA_LENGTHS * 2 + 2];  // slots by the time they become free, in order
+        int groups = 1;
+        double split = 0.0;  // pieces to be joined
+        at[0] = 0.0;
+        count[0] = slots;
+        for (int s = -1; s < n; ++s) {  // whole pieces first; lengths come in falling order
+            double items = 0.0, size = 0.0;
+            if (s >= 0 && len[s] > span) split += each * vspw_cdiv(len[s], span);
+            if (s < 0) {
+                for (int i = 0; i < n; ++i) items += each * (len[i] / span);
+                size = span + (p > 1 ? extra : 0);
+            } else if (len[s] % span) {
+                items = each;
+                size = len[s] % span + (len[s] > span ? extra : 0);
+            }
+            if (s < 0 && items > slots) {  // whole rounds
+                at[0] = floor(items / slots) * size;
+                items -= floor(items / slots) * slots;
+            }
+            while (items > 1e-6) {
+                const double take = items < count[0] ? items : count[0], t = at[0] + size;
+                items -= take;
+                count[0] -= take;
+                if (count[0] <= 1e-6) {
+                    --groups;
+                    for (int i = 0; i < groups; ++i) at[i] = at[i + 1], count[i] = count[i + 1];
+                }
+                int i = groups;
+                while (i > 0 && at[i - 1] > t) --i;
+                if (i > 0 && t - at[i - 1] < 0.5) {
+                    count[i - 1] += take;
+                    continue;
+                }
+                if (groups == (int)(sizeof(at) / sizeof(at[0]))) break;
+                for (int k = groups; k > i; --k) at[k] = at[k - 1], count[k] = count[k - 1];
+                at[i] = t;
+                count[i] = take;
+                ++groups;
+            }
+        }
+        const double c = at[groups - 1] + (split > 0.0 ? 1.0 + join * split / slots : 0.0);
+        if (c < cost * 0.98) {
+            cost = c;
+            best = p;
+        }
+    }
+    return best;
+}
 static int da_span(int n, int parts) { return vspw_cdiv(vspw_cdiv(n, DA_TILE), parts) * DA_TILE; }
 
 #define DA_NEAR (1LL << 24)  // elements: 64 rows of a tile times 4 bytes stay below 2^32
@@ -1297,17 +1414,49 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     // up to 32 rows: single-wave workgroups, many parts of the key axis; else four waves share a key tile
     p.wn = p.rows <= 32 ? 1 : 4;
     p.tiles = vspw_cdiv(p.rows, 32 * p.wn);
-    p.parts = p.wn == 1 ? da_parts(p.tiles * p.bhk, nt, 1024, 1, 256) : da_parts(p.tiles * p.bhk, nt, d->d == 64 ? 256 : 512, 4, 32);
+    const int slots = 256;
+    p.qt = vspw_cdiv(p.rows, 128);
+    p.kt = vspw_cdiv(d->nk, 128);
+    const int rt = vspw_cdiv(p.rows, DA_TILE), fslots = d->d == 64 ? 256 : 512;
+    if (p.wn == 1) {
+        p.parts = da_parts(p.tiles * p.bhk, nt, 1024, 1, 256);
+    } else {
+        p.parts = da_parts(p.tiles * p.bhk, nt, fslots, 4, 32);
+    }
+    p.qparts = da_parts(p.qt * p.bhk, nt, slots, 4, 16);
+    p.kparts = da_parts(p.kt * p.bhk, rt, slots, 4, 16);
+    if (d->frame > 0 && p.wn == 4) {
+        const double join = d->dtype == VSPW_F32 ? 0.8 : 2.5;  // reading a piece again, in tiles: bytes and fast products
+        int len[DA_LENGTHS];
+        bool even = true;
+        const long long shift = (long long)d->nk - d->nq;
+        int n = p.qt < DA_LENGTHS ? p.qt : DA_LENGTHS;
+        for (int s = 0; s < n; ++s) {
+            const long long tile = p.qt - 1 - (long long)(2 * s + 1) * p.qt / (2 * n), last = tile * 128 + 127;
+            const long long pos = (last < rows ? last : rows - 1) / p.g + shift;
+            const long long lim = pos < 0 ? 0 : (pos / d->frame + 1) * d->frame;
+            len[s] = vspw_cdiv(lim < d->nk ? lim : d->nk, DA_TILE);
+            even = even && len[s] == nt;
+        }
+        if (!even) {
+            p.parts = da_parts_frames(len, n, (double)p.qt * p.bhk / n, nt, fslots, 4, join, 32);
+            p.qparts = fslots == slots ? (p.parts < 16 ? p.parts : 16) : da_parts_frames(len, n, (double)p.qt * p.bhk / n, nt, slots, 4, join, 16);
+        }
+        even = true;
+        n = p.kt < DA_LENGTHS ? p.kt : DA_LENGTHS;
+        for (int s = 0; s < n; ++s) {
+            const long long key = (long long)(2 * s + 1) * p.kt / (2 * n) * 128, q0 = key / d->frame * d->frame - shift;
+            const long long r0 = q0 > 0 ? q0 * p.g / DA_TILE : 0;
+            len[s] = r0 < rt ? (int)(rt - r0) : 0;
+            even = even && len[s] == rt;
+        }
+        if (!even) p.kparts = da_parts_frames(len, n, (double)p.kt * p.bhk / n, rt, slots, 4, join, 16);
+    }
     p.span = da_span(d->nk, p.parts);
     p.parts = vspw_cdiv(d->nk, p.span);
     p.fwd_bytes = p.parts > 1 ? (size_t)p.parts * p.bhk * p.rows * (2 * W + 4) * sizeof(float) : 0;
-    const int slots = 256;
-    p.qt = vspw_cdiv(p.rows, 128);
-    p.qparts = da_parts(p.qt * p.bhk, nt, slots, 4, 16);
     p.qspan = da_span(d->nk, p.qparts);
     p.qparts = vspw_cdiv(d->nk, p.qspan);
-    p.kt = vspw_cdiv(d->nk, 128);
-    p.kparts = da_parts(p.kt * p.bhk, vspw_cdiv(p.rows, DA_TILE), slots, 4, 16);
     p.kspan = da_span(p.rows, p.kparts);
     p.kparts = vspw_cdiv(p.rows, p.kspan);
     const long long bh = (long long)d->b * d->h;
@@ -1417,8 +1566,8 @@ static int da_bwd_launch(DaArgs a, const DaPlan& p, hipStream_t st) {
         rc = vspw_launch_status();
         if (rc == VSPW_OK && p.qparts > 1) {
             const long long n = (long long)a.b * a.nq * a.h * 2 * D;
-            hipLaunchKernelGGL((da_sum_kernel<T>), dim3(vspw_stream_grid(n / 4, 256)), dim3(256), 0, st, a.part,
-                               reinterpret_cast<T*>(a.dq), n / 4, p.qparts, n);
+            hipLaunchKernelGGL((da_sum_kernel<T, false>), dim3(vspw_stream_grid(n / 4, 256)), dim3(256), 0, st, a,
+                               (const float*)a.part, reinterpret_cast<T*>(a.dq), n / 4, n, D / 2);
             rc = vspw_launch_status();
         }
     }
@@ -1430,12 +1579,12 @@ static int da_bwd_launch(DaArgs a, const DaPlan& p, hipStream_t st) {
         rc = vspw_launch_status();
         if (rc == VSPW_OK && p.kparts > 1) {
             const long long n = (long long)a.b * a.nk * a.hk * 2 * D;
-            hipLaunchKernelGGL((da_sum_kernel<T>), dim3(vspw_stream_grid(n / 4, 256)), dim3(256), 0, st, a.part,
-                               reinterpret_cast<T*>(a.dk), n / 4, p.kparts, 2 * n);
+            hipLaunchKernelGGL((da_sum_kernel<T, true>), dim3(vspw_stream_grid(n / 4, 256)), dim3(256), 0, st, a,
+                               (const float*)a.part, reinterpret_cast<T*>(a.dk), n / 4, 2 * n, D / 2);
             rc = vspw_launch_status();
             if (rc == VSPW_OK)
-                hipLaunchKernelGGL((da_sum_kernel<T>), dim3(vspw_stream_grid(n / 4, 256)), dim3(256), 0, st, a.part + n,
-                                   reinterpret_cast<T*>(a.dv), n / 4, p.kparts, 2 * n);
+                hipLaunchKernelGGL((da_sum_kernel<T, true>), dim3(vspw_stream_grid(n / 4, 256)), dim3(256), 0, st, a,
+                                   (const float*)(a.part + n), reinterpret_cast<T*>(a.dv), n / 4, 2 * n, D / 2);
             if (rc == VSPW_OK) rc = vspw_launch_status();
         }
     }

@@ -147,6 +147,15 @@ def test_frames(dev, dt, nq, nk, frame):
 
 
 @pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("nq,nk,frame,d", [(1500, 1500, 250, 64), (900, 2100, 300, 16), (2000, 700, 100, 32), (700, 1400, 1, 64),
+                                           (130, 5000, 65, 32)])
+def test_frames_in_parts(dev, dt, nq, nk, frame, d):
+    """Long enough that tiles stream different numbers of parts, one of them or none; with keys hidden as well."""
+    mask = torch.rand(1, nk, generator=torch.Generator().manual_seed(nk)) < 0.7
+    run_case(dev, *inputs(1, nq, nk, 2, 1, d, dt), mask, frame=frame)
+
+
+@pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("d", [16, 32, 64])
 def test_masks(dev, dt, d):
     """A batch entry without any key, one with a single key, one with alternating keys; then together with frames."""
