@@ -620,6 +620,8 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
     }
 }
 
+#define DA_JOIN_PARTS 32
+#define DA_ROW_PARTS 512
 // Joins the parts of a row.  Up to 32 parts: W / 4 threads per row, each goes over the parts by itself (every thread of a row
 // reads the same maxima and sums of weights, from the cache).
 __device__ __forceinline__ int da_last_of(const DaArgs& a, int row) {  // the last row of the forward kernel's tile
@@ -668,62 +670,75 @@ __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
     }
 }
 
-// More parts (few rows, a long axis): one workgroup per row, the parts dealt out over its threads, sums in a fixed tree.
+// More parts (few rows, a long axis): a workgroup takes 8 columns of both maps of a row and deals the parts out over 64 groups
+// of its threads, sums in a fixed tree.  4 rows of 394 parts: FIGURES.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void da_join_row_kernel(const DaArgs a) {
-    constexpr int W = 2 * D, CT = 2 * W / 4, PT = 256 / CT;  // CT threads hold one part's two sums
+    constexpr int W = 2 * D, COLS = 8, CT = 2 * COLS / 4, PT = 256 / CT;  // CT threads hold one part's columns of both maps
     __shared__ float red[4][4];
-    __shared__ f32x4 sum[256];
+    __shared__ f32x4 sum[4][CT];
     const int tid = threadIdx.x, wave = tid >> 6;
-    const size_t n = (size_t)a.b * a.hk * a.rows, e = blockIdx.x;
+    const size_t n = (size_t)a.b * a.hk * a.rows, e = blockIdx.x / (W / COLS);
+    const int col0 = blockIdx.x % (W / COLS) * COLS;
     const int bh = (int)(e / a.rows), row = (int)(e % a.rows);
     const int head = (bh % a.hk) * a.g + row % a.g;
     const int nparts = da_row_parts(a, da_last_of(a, row));
     if (nparts == 1) return;
-    const f32x4 none = {-DA_INF, 0.f, -DA_INF, 0.f};
-    const f32x4 mine = tid < nparts ? *reinterpret_cast<const f32x4*>(a.ml + (tid * n + e) * 4) : none;  // at most 256 parts
-    float u[2], L[2];
-    const float w1 = wave_max(mine[0]), w2 = wave_max(mine[2]);
-    if ((tid & 63) == 0) {
-        red[0][wave] = w1;
-        red[1][wave] = w2;
+    f32x4 mine[DA_ROW_PARTS / 256];
+    float u[2] = {-DA_INF, -DA_INF}, L[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < DA_ROW_PARTS / 256; ++i) {
+        const int p = tid + 256 * i;
+        mine[i] = p < nparts ? *reinterpret_cast<const f32x4*>(a.ml + (p * n + e) * 4) : f32x4{-DA_INF, 0.f, -DA_INF, 0.f};
+        u[0] = fmaxf(u[0], mine[i][0]);
+        u[1] = fmaxf(u[1], mine[i][2]);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        u[m] = wave_max(u[m]);
+        if ((tid & 63) == 0) red[m][wave] = u[m];
     }
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         u[m] = fmaxf(fmaxf(red[m][0], red[m][1]), fmaxf(red[m][2], red[m][3]));
         if (u[m] == -DA_INF) u[m] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DA_ROW_PARTS / 256; ++i) L[m] = fmaf(mine[i][2 * m + 1], exp2f(mine[i][2 * m] - u[m]), L[m]);
+        L[m] = wave_sum(L[m]);
+        if ((tid & 63) == 0) red[2 + m][wave] = L[m];
     }
-    const float s1 = wave_sum(mine[1] * exp2f(mine[0] - u[0])), s2 = wave_sum(mine[3] * exp2f(mine[2] - u[1]));
-    if ((tid & 63) == 0) {
-        red[2][wave] = s1;
-        red[3][wave] = s2;
-    }
-    const int ch = tid % CT, map = ch >= CT / 2 ? 1 : 0;
+    const int c = tid % CT, map = c / (CT / 2), ch = map * W + col0 + c % (CT / 2) * 4;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = tid / CT; p < nparts; p += PT)
-        acc += *reinterpret_cast<const f32x4*>(a.part + (p * n + e) * 2 * W + 4 * ch) * exp2f(a.ml[(p * n + e) * 4 + 2 * map] - u[map]);
-    sum[tid] = acc;
+#pragma unroll
+    for (int i = 0; i < DA_ROW_PARTS / PT; ++i) {
+        const int p = tid / CT + PT * i;
+        if (p < nparts)
+            acc += *reinterpret_cast<const f32x4*>(a.part + (p * n + e) * 2 * W + ch) *
+                   exp2f(a.ml[(p * n + e) * 4 + 2 * map] - u[map]);
+    }
+#pragma unroll
+    for (int s = CT; s < 64; s *= 2)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor(acc[x], s, 64);
+    if ((tid & 63) < CT) sum[wave][c] = acc;
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < 2; ++m) L[m] = (red[2 + m][0] + red[2 + m][1]) + (red[2 + m][2] + red[2 + m][3]);
     if (tid < CT / 2) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-        for (int p = 0; p < PT; ++p) {
-            x += sum[p * CT + tid];
-            y += sum[p * CT + CT / 2 + tid];
-        }
+        f32x4 x = (sum[0][tid] + sum[1][tid]) + (sum[2][tid] + sum[3][tid]);
+        f32x4 y = (sum[0][CT / 2 + tid] + sum[1][CT / 2 + tid]) + (sum[2][CT / 2 + tid] + sum[3][CT / 2 + tid]);
         x = da_scaled(x, L[0] == 0.f ? 0.f : 1.f / L[0]);
         y = da_scaled(y, L[1] == 0.f ? 0.f : 1.f / L[1]);
         const size_t o = (((size_t)(bh / a.hk) * a.nq + row / a.g) * a.h + head) * W;
-        Mx<T>::store4(reinterpret_cast<T*>(a.out) + o + 4 * tid, da_mix(x, y, da_lambda(a, head)));
+        const int oc = col0 + 4 * tid;
+        Mx<T>::store4(reinterpret_cast<T*>(a.out) + o + oc, da_mix(x, y, da_lambda(a, head)));
         if (a.maps) {
-            *reinterpret_cast<f32x4*>(a.maps + 2 * o + 4 * tid) = x;
-            *reinterpret_cast<f32x4*>(a.maps + 2 * o + W + 4 * tid) = y;
+            *reinterpret_cast<f32x4*>(a.maps + 2 * o + oc) = x;
+            *reinterpret_cast<f32x4*>(a.maps + 2 * o + W + oc) = y;
         }
     }
-    if (a.lse && tid < 2) a.lse[tid * n + e] = L[tid] == 0.f ? DA_INF : u[tid] + log2f(L[tid]);
+    if (a.lse && col0 == 0 && tid < 2) a.lse[tid * n + e] = L[tid] == 0.f ? DA_INF : u[tid] + log2f(L[tid]);
 }
 
 // --------------------------------------------------------------------------------------------------------- backward
@@ -1316,13 +1331,15 @@ __global__ __launch_bounds__(64) void diff_lambda_kernel(const float* __restrict
 static int da_parts(long long nb, int nt, int slots, int extra, int most) {
     int best = 1;
     double cost = 1e300;
-    for (int p = 1; p <= most && p <= nt; ++p) {
+    for (int p = 1, len = nt; p <= most; len = vspw_cdiv(nt, p)) {  // the fewest parts for each length
         const long long rounds = (nb * p + slots - 1) / slots;
-        const double c = (double)rounds * ((nt + p - 1) / p + (p > 1 ? extra : 0)) + (p > 1 ? 0.02 * p : 0.0);
+        const double c = (double)rounds * (len + (p > 1 ? extra : 0)) + (p > 1 ? 0.02 * p : 0.0);
         if (c < cost * 0.98) {
             cost = c;
             best = p;
         }
+        if (len == 1) break;
+        p = vspw_cdiv(nt, len - 1);
     }
     return best;
 }
@@ -1419,7 +1436,7 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     p.kt = vspw_cdiv(d->nk, 128);
     const int rt = vspw_cdiv(p.rows, DA_TILE), fslots = d->d == 64 ? 256 : 512;
     if (p.wn == 1) {
-        p.parts = da_parts(p.tiles * p.bhk, nt, 1024, 1, 256);
+        p.parts = da_parts(p.tiles * p.bhk, nt, 1024, 1, DA_ROW_PARTS);
     } else {
         p.parts = da_parts(p.tiles * p.bhk, nt, fslots, 4, 32);
     }
@@ -1466,7 +1483,7 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     if (lc < 1) lc = 1;
     p.lchunks = (int)lc;
     if (p.tiles * p.bhk * p.parts > INT_MAX || p.qt * p.bhk * p.qparts > INT_MAX || p.kt * p.bhk * p.kparts > INT_MAX ||
-        bh * p.lchunks > INT_MAX || p.bhk * p.rows > INT_MAX)
+        bh * p.lchunks > INT_MAX || p.bhk * p.rows > INT_MAX || (p.parts > DA_JOIN_PARTS && p.bhk * p.rows * (W / 8) > INT_MAX))
         return false;
     size_t parts = 0;  // dq and dk/dv run one after the other and share the partial sums' memory
     if (p.qparts > 1) parts = (size_t)p.qparts * p.bhk * p.rows * W;
@@ -1531,8 +1548,6 @@ extern "C" size_t vspw_diff_attn_bwd_workspace(const vspw_dattn_desc* d) {
     return da_plan(d, p) ? p.bwd_bytes : 0;
 }
 
-#define DA_JOIN_PARTS 32
-
 template <typename T, int D>
 static int da_fwd_launch(const DaArgs& a, const DaPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)(p.tiles * p.bhk * p.parts));
@@ -1544,7 +1559,7 @@ static int da_fwd_launch(const DaArgs& a, const DaPlan& p, hipStream_t st) {
     if (rc != VSPW_OK || p.parts == 1) return rc;
     const long long rows = p.bhk * p.rows;
     if (p.parts > DA_JOIN_PARTS)
-        hipLaunchKernelGGL((da_join_row_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((da_join_row_kernel<T, D>), dim3((unsigned)(rows * (2 * D / 8))), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((da_join_kernel<T, D>), dim3((unsigned)vspw_cdiv(rows, 256 / (D / 2))), dim3(256), 0, st, a);
     return vspw_launch_status();

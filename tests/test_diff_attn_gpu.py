@@ -134,6 +134,7 @@ def run_case(dev, q, k, v, lam, go, mask=None, frame=0, scale=None, place=lambda
 @pytest.mark.parametrize("case", [
     (1, 1, 1, 1, 1, 16), (1, 1, 2, 1, 1, 32), (2, 3, 31, 2, 2, 32), (1, 32, 32, 1, 1, 64), (2, 33, 33, 1, 1, 16),
     (1, 65, 64, 2, 1, 32), (1, 129, 127, 2, 2, 64), (2, 300, 257, 4, 2, 16), (1, 7, 130, 8, 2, 64), (2, 200, 5, 3, 1, 32),
+    (1, 1, 25200, 4, 1, 64), (1, 3, 17000, 2, 2, 16), (2, 2, 7000, 2, 1, 32),
     (1, 40, 700, 2, 2, 32), (1, 1, 1500, 4, 1, 64), (2, 1, 999, 2, 2, 16), (1, 500, 40, 4, 1, 64)])
 def test_sizes_and_heads(dev, dt, case):
     run_case(dev, *inputs(*case, dt))
