@@ -3,6 +3,8 @@
 // word per image and channel: nn.Dropout2d).  The backward pass is the same call on the gradient.
 //
 // Bound: HBM (one read, one write).  The generator costs 20 32x32->64 multiplies per four elements.
+// Measured: [2,4096,60,60] fp32, 118 MB in and out: 41 us, 5.7 TB/s; channel form, [10,2048,60,60] bf16, 147 MB in and out: 57 us,
+// 5.2 TB/s.
 #include "elem.h"
 
 // Element form.  One trip handles 16 bytes (VEC) or the same elements one by one (ragged tail, unaligned storage).

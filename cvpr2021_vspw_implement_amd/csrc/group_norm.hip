@@ -8,7 +8,9 @@
 // from zero costs no digits.  The mean enters the fp32 arithmetic as two terms; ReLU's border is decided on the fp64
 // pre-activation (the same in both directions).  All sums have a fixed order: results are bit-reproducible.
 //
-// Large images: streaming kernels, stats -> finish -> apply and bwd_stats -> bwd_reduce -> bwd_apply, bound by HBM.  Images whose
+// Large images: streaming kernels, stats -> finish -> apply and bwd_stats -> bwd_reduce -> bwd_apply, bound by HBM.
+// [10,512,60,60] fp32 (74 MB), ReLU, dropout: 26 (2.8 TB/s, x comes from memory) + 4 + 28 us (5.3 TB/s), 30 (5.0) + 5 + 38 us
+// (5.9 TB/s); [4,256,119,119] bf16 (29 MB), SiLU: 12 + 4 + 16, 21 + 5 + 21 us.  The two small kernels cost a launch each.  Images whose
 // groups fit the registers of a workgroup: one workgroup per image and group, which reads its elements once.
 #include <type_traits>
 
