@@ -103,6 +103,14 @@ struct IgemmNT {
 #endif
 };
 
+// The edge epilogues' sums of squares: which products are rounded before they are added is written out, so that it does not
+// depend on the instructions the compiler may use (without packed ones it would fuse all of them, and the training steps that
+// are compared with the full-size reference vectors would take another rounding path).
+template <typename V>
+__device__ __forceinline__ V rounded_product(V a, V b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 __device__ __forceinline__ float nt_act(float v, int act) {
     if (act == 1) return fmaxf(v, 0.f);
     if (act == 2) return 1.f / (1.f + expf(-v));
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(256) void igemm_nt_kernel(IgemmNT pin) {
                     const float v = nt_act(t, p.act);  // act(conv + bias + addend): residual add, then ReLU
                     p.dst[(size_t)row * p.ldd + col] = v;
                     csum[j] += v;
-                    csq[j] += v * v;
+                    csq[j] = WN == 2 ? fmaf(v, v, csq[j]) : csq[j] + rounded_product(v, v);
                 }
             }
         }
@@ -1042,7 +1050,7 @@ __device__ __forceinline__ void igemm_nt_v2_body(const IgemmNT& pin, int vb_in, 
                         }
                         p.dst[(size_t)row * p.ldd + col] = v;
                         csum[j] += v;
-                        csq[j] += v * w2;
+                        csq[j] += rounded_product(v, w2);
                     }
                 }
             }

@@ -13,14 +13,14 @@ from ._metrics import pixel_accuracy
 
 
 class Non_local3d(LrGroupsMixin, nn.Module):
-    def __init__(self, args, net_enc, crit, downsample=False):
-        """args.nl_mode: mode of the non-local block (default 'dot', the reference's; see NLBlockND)."""
+    def __init__(self, args, net_enc, crit, downsample=False, nl_mode="dot"):
+        """nl_mode: mode of the non-local block ('dot' is the reference's; see NLBlockND)."""
         super().__init__()
         self.encoder = net_enc
         self.downsample = downsample
         self.crit = crit
         self.emb = vnn.Conv2d(2048, 256, 1, 1)
-        self.nonlocalblock = NLBlockND(in_channels=256, mode=getattr(args, "nl_mode", "dot"), dimension=3, bn_layer=True)
+        self.nonlocalblock = NLBlockND(in_channels=256, mode=nl_mode, dimension=3, bn_layer=True)
         self.last_layer = vnn.Conv2d(512, args.num_class, kernel_size=1, stride=1)
 
     def _lr_10x_roots(self):

@@ -9,8 +9,9 @@ There is no CPU fallback: a CPU tensor raises (SURVEY.md §8b "Errors").
 
 Layout of the module family: _opbase.py (pointer / layout helpers, launch timers), _ops_conv.py (convolutions, Winograd
 dispatch, derived-weight caches), _ops_bn.py (BatchNorm, conv+BN+activation nodes), _ops_norm.py (GroupNorm+activation,
-counter-based dropout: also bfloat16 / float16), _ops_attn.py (differential attention: also bfloat16); this file holds the remaining operators (pooling, interpolation, losses, batched GEMMs, non-local, flow) and re-exports the others, so callers keep
-using `ops.<name>`.
+counter-based dropout: also bfloat16 / float16), _ops_attn.py (differential attention: also bfloat16); this file holds
+the remaining operators (pooling, interpolation, losses, batched GEMMs, non-local, flow) and re-exports the others, so
+callers keep using `ops.<name>`.
 """
 import ctypes
 import os

@@ -202,8 +202,6 @@ def build_parser():
     p.add_argument("--vc_clip_num", type=int, default=8)
     p.add_argument("--psp_weight", type=str2bool, default=False)
     p.add_argument("--raft_weights", type=str, default="")  # NetWarp's RAFT comes from --load; no separate file needed
-    p.add_argument("--nl_mode", default="dot", choices=["dot", "differential"],
-                   help="affinity of the nonlocal3d block: the reference's dot product or the difference of two softmax maps")
     p.add_argument("opts", help="Modify config options using the command-line", default=None, nargs=argparse.REMAINDER)
     return p
 

@@ -47,7 +47,8 @@ def build_module(cfg, args, num_class, training=True):
     if args.method == "netwarp":
         return NetWarp(enc, dec, crit, args, cfg.TRAIN.deep_sup_scale)
     if args.method == "nonlocal3d":
-        return Non_local3d(args, enc, crit)
+        # the decoder of this method is the block itself: a differential decoder in the config selects its kind
+        return Non_local3d(args, enc, crit, nl_mode="differential" if "differential" in cfg.MODEL.arch_decoder.lower() else "dot")
     if args.method == "clip_psp":
         return Clip_PSP(enc, crit, args, deep_sup_scale=ds)
     if args.method == "clip_ocr":
@@ -415,8 +416,6 @@ def build_parser():
                    help="replay the training step as one captured hipGraph (fixed crop / batch shapes; no reference "
                         "counterpart)")
     p.add_argument("--raft_weights", type=str, default="./RAFT_core/raft-things.pth-no-zip")
-    p.add_argument("--nl_mode", default="dot", choices=["dot", "differential"],
-                   help="affinity of the nonlocal3d block: the reference's dot product or the difference of two softmax maps")
     p.add_argument("opts", help="Modify config options using the command-line", default=None, nargs=argparse.REMAINDER)
     return p
 

@@ -150,7 +150,7 @@ def test_decoders(dev):
             return [x]
 
     crit = torch.nn.NLLLoss(ignore_index=255)
-    head = M.Non_local3d(args_ns(num_class=12, nl_mode="differential"), Enc(), crit).to(dev)
+    head = M.Non_local3d(args_ns(num_class=12), Enc(), crit, nl_mode="differential").to(dev)
     clip = [torch.randn(1, 2048, 6, 7, device=dev) for _ in range(3)]
     labs = [torch.randint(0, 12, (1, 1, 48, 56), device=dev).float() for _ in range(3)]
     loss, _ = head({"clipimgs_data": clip, "cliplabels_data": labs})
