@@ -373,8 +373,8 @@ struct RowOf {
 
 // ---------------------------------------------------------------------------------------------------------- forward
 // Software pipeline.  A: the scores of tile t + 1 on the matrix unit, tile t's weights 2^(c S - m) on the vector unit; B: tile
-// t's weights times v, and the maximum of tile t + 1.  One barrier per tile, between A and B; the operands that follow it were
-// read before it.  k of tile t + 2 is put into LDS in A (its buffer was last read in the A before), v of tile t + 1 in B.
+// t's weights times v, and the maximum of tile t + 1.  One barrier per tile, between A and B.  k of tile t + 2 is put into
+// LDS in A (its buffer was last read in the A before), v of tile t + 1 in B: both are read behind the next barrier only.
 // Four waves of 32 rows share a key tile; up to 32 rows are one wave, and the keys are cut into more parts instead.
 // Measured (12 D operations per row and key): fp32, 2 x 18000 rows and keys, D = 64: 4.33 ms, 115 TFLOP/s, matrix unit busy
 // 76 - 80 %, its rate is the bound.  bf16, 6420 rows and keys, 4 heads, D = 32: 154 us, 411 TFLOP/s (the second term of the
@@ -492,8 +492,8 @@ __global__ __launch_bounds__(64 * WN, WN == 1 || D == 64 ? 1 : 2) void da_fwd_ke
                 da_pin();
             }
         }
-        Frag vn = M::col(Vs[cur], LD, 0, 0, lane);
         __syncthreads();
+        Frag vn = M::col(Vs[cur], LD, 0, 0, lane);  // put by all waves in the B before
         da_pin();
         x1 = x2 = -DA_INF;
         constexpr int SB = 2 * CB * M::RSTEPS, S0 = SB >= 16 ? 2 : 0;  // the scores' last products are still in flight

@@ -355,6 +355,22 @@ def test_refusals(dev):
         ops.diff_lambda(lam, lam, lam, lam, 0.1)
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("case", [(1, 1152, 1152, 4, 2, 16), (2, 700, 900, 2, 1, 32), (1, 600, 1300, 2, 2, 64)])
+def test_waves_of_a_workgroup_wait_for_each_other(dev, dt, case):
+    """Workgroups of four waves on short tiles: the values, and the same bits from every run."""
+    from cvpr2021_vspw_implement_amd import ops
+
+    q, k, v, lam, go = inputs(*case, dt)
+    out, leaves = run_case(dev, q, k, v, lam, go)
+    qd, kd, vd, ld = (t.detach().requires_grad_(True) for t in leaves)
+    god = go.to(dev)
+    for _ in range(40):
+        again = ops.diff_attention(qd, kd, vd, ld)
+        assert torch.equal(again, out)
+        assert all(torch.equal(g, t.grad) for g, t in zip(torch.autograd.grad(again, (qd, kd, vd, ld), god), leaves))
+
+
 def test_a_second_derivative_is_refused(dev):
     from cvpr2021_vspw_implement_amd import ops
 
