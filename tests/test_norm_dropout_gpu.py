@@ -436,3 +436,24 @@ def test_empty(dev, shape):
         assert y.shape == shape
         gx, gw = torch.autograd.grad(y.sum(), (x, w))
         assert gx.shape == shape and (gw == 0).all()
+
+
+def test_broadcast_inputs(dev):
+    """An input that is an expanded row: the gradient comes back summed over the broadcast dimensions."""
+    from cvpr2021_vspw_implement_amd import ops
+
+    rng = make_rng(dev, 4)
+    row = torch.randn(1, 8, 1, 6, device=dev)
+    w = torch.randn(1, device=dev)
+    gy = torch.randn(3, 8, 5, 6, device=dev)
+    grads = []
+    for expanded in (True, False):
+        r, wl = row.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        x, we = r.expand(3, 8, 5, 6), wl.expand(8)
+        if not expanded:
+            x, we = x.contiguous(), we.contiguous()
+        y = ops.group_norm_act(x, 2, we, None, act="gelu", p=0.25, rng=rng)
+        grads.append((y,) + torch.autograd.grad(y, (r, wl), gy))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    x = row.expand(3, 8, 5, 6)
+    assert torch.equal(ops.dropout(x, 0.25, rng), ops.dropout(x.contiguous(), 0.25, rng))
