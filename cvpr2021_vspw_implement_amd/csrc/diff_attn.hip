@@ -171,6 +171,7 @@ struct DaArgs {
     float* part;                // partial results of a split axis
     float* ml;                  // forward: [chunks][B*Hk][rows][2] running maximum and sum per map: [..][2 m], [..][2 m + 1]
     double* lpart;              // [B*H][lchunks]: sums of D_2
+    int* alone;                 // [B]: at most one key takes part
     long long q_sb, q_sn, q_sh, q_sm, k_sb, k_sn, k_sh, k_sm, v_sb, v_sn, v_sh;
     int b, nq, nk, h, hk, g, rows, frame, lam_bf16, lchunks;
     int tiles, parts, span;     // workgroups along the owned axis; split of the streamed axis: parts of `span` entries
@@ -759,6 +760,20 @@ __global__ __launch_bounds__(256) void da_delta_kernel(const DaArgs a) {
     const int sub = threadIdx.x % LPR;
     const float lam = da_lambda(a, head);
     const size_t n = (size_t)a.b * a.hk * a.rows;
+    if (chunk == 0 && head == 0) {  // counts the keys that take part, up to two
+        int seen = a.mask ? 0 : a.nk;
+        const unsigned char* m = a.mask ? a.mask + (size_t)bi * a.nk : nullptr;
+        for (int j0 = 0; m && j0 < a.nk && seen < 2; j0 += 16 * 256) {
+            int here = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = j0 + 256 * i + (int)threadIdx.x;
+                here += (j < a.nk) & (m[min(j, a.nk - 1)] != 0);
+            }
+            seen += __syncthreads_count(here == 1) + 2 * (__syncthreads_count(here > 1) != 0);
+        }
+        if (threadIdx.x == 0) a.alone[bi] = seen < 2;
+    }
     double total = 0.0;
     for (int q = chunk * (256 / LPR) + threadIdx.x / LPR; q < a.nq; q += a.lchunks * (256 / LPR)) {
         const size_t o = (((size_t)bi * a.nq + q) * a.h + head) * W;
@@ -999,12 +1014,14 @@ __global__ __launch_bounds__(256, D >= 32 ? 1 : 2) void da_dq_kernel(const DaArg
     }
     if (!ro.live) return;
     const float f2 = -da_lambda(a, ro.head) * a.scale;
+    const bool alone = a.alone[ro.bi] != 0;  // the softmax of one key is constant: exactly no gradient
 #pragma unroll
     for (int j = 0; j < DB; ++j)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
             const int ch = 32 * j + 8 * g4 + 4 * lh;
-            const f32x4 x = quad(g1[j], g4) * a.scale, y = quad(g2[j], g4) * f2;
+            f32x4 x = quad(g1[j], g4) * a.scale, y = quad(g2[j], g4) * f2;
+            if (alone) x = y = f32x4{0.f, 0.f, 0.f, 0.f};
             // D = 16: map 1 sits in channels 0..15 of its product, map 2 in channels 16..31 of its own
             const bool ok1 = D >= 32 || ch < D, ok2 = D >= 32 || ch >= D;
             if (nparts > 1) {
@@ -1264,8 +1281,9 @@ __global__ __launch_bounds__(256, 1) void da_dkv_kernel(const DaArgs a) {
     if (key >= a.nk) return;
     const size_t o = (((size_t)bi * a.nk + key) * a.hk + kh) * W;
     const size_t all = (size_t)a.b * a.nk * a.hk * W;
+    const bool alone = a.alone[bi] != 0;  // the softmax of one key is constant: exactly no gradient
     auto out = [&](int which, int ch, f32x4 x) {
-        if (!live) x = f32x4{0.f, 0.f, 0.f, 0.f};  // whatever a hidden key's column holds, it never left this lane
+        if (!live || (alone && which == 0)) x = f32x4{0.f, 0.f, 0.f, 0.f};  // whatever a hidden key's column holds, it never left this lane
         if (part0 + 1 < a.parts)
             *reinterpret_cast<f32x4*>(a.part + ((size_t)part * 2 + which) * all + o + ch) = x;
         else
@@ -1499,7 +1517,7 @@ static bool da_plan(const vspw_dattn_desc* d, DaPlan& p) {
     if (p.qparts > 1) parts = (size_t)p.qparts * p.bhk * p.rows * W;
     if (p.kparts > 1 && (size_t)p.kparts * 2 * p.bhk * d->nk * W > parts) parts = (size_t)p.kparts * 2 * p.bhk * d->nk * W;
     p.bwd_bytes = (size_t)bh * p.lchunks * sizeof(double) + ((size_t)6 * p.bhk * p.rows + parts) * sizeof(float);
-    p.bwd_bytes += 32;  // alignment of the pieces
+    p.bwd_bytes += (size_t)d->b * sizeof(int) + 48;  // alone; alignment of the pieces
     return true;
 }
 static bool da_strides_ok(const vspw_dattn_desc* d, const DaPlan& p, const void* q, const void* k, const void* v) {
@@ -1659,11 +1677,13 @@ extern "C" int vspw_diff_attn_bwd(const vspw_dattn_desc* d, const void* q, const
     a.dk = dk;
     a.dv = dv;
     a.dlam = dlam;
-    // [lpart doubles][stat][partial sums], every piece on 16 bytes
+    // [lpart doubles][stat][alone][partial sums], every piece on 16 bytes
     a.lpart = reinterpret_cast<double*>(ws);
     size_t off = ((size_t)d->b * d->h * p.lchunks * sizeof(double) + 15) / 16 * 16;
     a.stat = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + off);
     off += ((size_t)6 * p.bhk * p.rows * sizeof(float) + 15) / 16 * 16;
+    a.alone = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + off);
+    off += ((size_t)d->b * sizeof(int) + 15) / 16 * 16;
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + off);
     return DA_DISPATCH(da_bwd_launch, a, p, vspw_stream(stream));
 }

@@ -440,3 +440,16 @@ def test_two_threads(dev):
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("nq,nk,keys", [(1, 1, None), (70, 1, None), (300, 40, [17]), (5, 9000, [4097]), (140, 9000, []), (3, 9000, [0, 8999])])
+def test_a_single_key_has_no_score_gradient(dev, dt, nq, nk, keys):
+    """The softmax of one key is 1 whatever the score: dq and dk are zero, not rounding; two keys are an ordinary case."""
+    mask = None
+    if keys is not None:
+        mask = torch.zeros(2, nk, dtype=torch.bool)
+        mask[:, keys] = True
+    out, (q, k, v, lam) = run_case(dev, *inputs(2, nq, nk, 2, 1, 16, dt), mask)
+    few = nk == 1 or (keys is not None and len(keys) < 2)
+    assert bool((q.grad == 0).all()) == few and bool((k.grad == 0).all()) == few
