@@ -781,11 +781,11 @@ __global__ __launch_bounds__(256) void da_delta_kernel(const DaArgs a) {
         Vec<T, V>::load(reinterpret_cast<const T*>(a.go) + o + V * sub, go);
         const f32x4 x = *reinterpret_cast<const f32x4*>(a.maps + 2 * o + V * sub);
         const f32x4 y = *reinterpret_cast<const f32x4*>(a.maps + 2 * o + W + V * sub);
-        float d1 = 0.f, d2 = 0.f;
+        double d1 = 0.0, d2 = 0.0;  // dlam's sum over the rows may cancel: nothing is rounded on the way to it
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            d1 = fmaf(go[i], x[i], d1);
-            d2 = fmaf(go[i], y[i], d2);
+            d1 = fma((double)go[i], (double)x[i], d1);
+            d2 = fma((double)go[i], (double)y[i], d2);
         }
         for (int s = LPR / 2; s > 0; s >>= 1) {
             d1 += __shfl_xor(d1, s, 64);
@@ -796,11 +796,11 @@ __global__ __launch_bounds__(256) void da_delta_kernel(const DaArgs a) {
             const size_t e = ((size_t)bi * a.hk + kh) * a.rows + row;
             a.stat[e] = a.lse[e];
             a.stat[n + e] = a.lse[n + e];
-            a.stat[2 * n + e] = d1;
-            a.stat[3 * n + e] = d2;
+            a.stat[2 * n + e] = (float)d1;
+            a.stat[3 * n + e] = (float)d2;
             a.stat[4 * n + e] = lam;
             a.stat[5 * n + e] = __int_as_float(da_limit(a, row));
-            total += (double)d2;
+            total += d2;
         }
     }
     total = wave_sum_d(total);
